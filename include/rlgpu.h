@@ -378,6 +378,58 @@ int rlgpu_lt_write_adam(const char* path, const int32_t* dims, int n_linear, flo
 int rlgpu_lt_read_adam(const char* path, const int32_t* dims, int n_linear, float* exp_avg, float* exp_avg_sq, int64_t* step);
 const char* rlgpu_lt_last_error(void);
 
+/* ---- operators for a policy network of the caller's own (csrc/rlgpu_ops.hip) -------------------------------------------------------------
+ * What stands around such a network's matrix products in an update: log-probabilities and entropy of given actions with their gradient, the clipped
+ * policy loss with a KL term with its gradient, the norm over all gradient tensors and the clip.  rlgpu_ppo_minibatch / rlgpu_clip_adam_step do the
+ * same work inside the library's own MLPs.  There is no handle: every pointer is the caller's (device memory unless it says host), every launch goes to
+ * `hip_stream` on `device`, nothing is kept between calls and nothing synchronises, so calls may be captured into graphs and may run at once on several
+ * streams as long as each has a workspace of its own.  The text of an error: rlgpu_ops_last_error() (of the calling thread). */
+enum { RLGPU_F32 = 0, RLGPU_BF16 = 1, RLGPU_F16 = 2 };
+typedef struct RlgpuPolicyRows {
+    const void* logits; int64_t ld;           /* [rows][n_actions], row stride `ld` in elements (>= n_actions), any alignment of a row */
+    const uint8_t* mask; int64_t ld_mask;     /* optional [rows][n_actions]: 0 = the action is not allowed, its logit is not looked at (it may be NaN); ld_mask 0: one row for all */
+    const int32_t* actions;                   /* [rows]; an index outside 0 .. n_actions - 1 leaves the row out */
+    int32_t dtype, rows, n_actions;           /* RLGPU_F32 / BF16 / F16, rows >= 0, 1 <= n_actions <= 2^28 */
+    float temperature, min_prob;              /* > 0; the floor of a probability, 0 < min_prob < 1 (rlgpu_policy_act: 1e-11) */
+} RlgpuPolicyRows;
+/* Per row, over the allowed actions, with s = softmax(logits / temperature):
+ *   logp = log max(s[action], min_prob)   (an action that is not allowed has s = 0),   entropy = -sum s log s   (0 log 0 = 0).
+ * A row is LEFT OUT when its action is out of range or when nothing is allowed in it (mask all 0, or every allowed logit -inf or the type's lowest finite
+ * value): logp = entropy = 0 and its gradient is zero.  NaN and +inf among the allowed logits give NaN; finite logits are taken up to |logit| / temperature < 2e38.
+ * entropy may be NULL.  Workspace: rlgpu_policy_workspace bytes, 16-byte aligned, free again when the call's work on the stream is done. */
+int64_t rlgpu_policy_workspace(int32_t dtype, int32_t rows, int32_t n_actions);   /* bytes, for any of the three calls below; < 0: bad argument */
+int rlgpu_action_logp(int device, const RlgpuPolicyRows* p, float* logp, float* entropy, void* workspace, int64_t workspace_bytes, void* hip_stream);
+/* dlogits[rows][n_actions] (p->dtype, row stride ld_dlogits) = d(sum d_logp logp + d_entropy entropy) / d logits; d_entropy may be NULL (zero).  The floor
+ * passes no gradient, actions that are not allowed get 0.  dlogits may be p->logits itself (same stride), else the two may not overlap. */
+int rlgpu_action_logp_backward(int device, const RlgpuPolicyRows* p, const float* d_logp, const float* d_entropy, void* dlogits, int64_t ld_dlogits,
+                               void* workspace, int64_t workspace_bytes, void* hip_stream);
+/* loss = scale * sum over rows of w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - 1 - d) - ent_coef entropy),
+ *   r = exp(logp - old_logp), d = ref_logp - logp (the KL term: an estimate of KL(policy || reference) from the taken action that is never negative), and
+ * dlogits = its gradient, in one pass.  Where the clipped term is the smaller one no gradient flows through r (rlgpu_ppo_minibatch's rule).
+ * weights NULL = 1; a row with weight 0 is left out too, and nothing else of it is looked at. */
+typedef struct RlgpuPolicyLoss {
+    const float *old_logp, *adv;              /* [rows] */
+    const float *ref_logp, *weights;          /* [rows], optional; ref_logp is needed when kl_coef != 0 */
+    float clip_low, clip_high;                /* 0 <= clip_low < 1, 0 <= clip_high */
+    float ent_coef, kl_coef, scale;           /* finite; scale is e.g. loss scale / rows of the batch */
+    float* logp;                              /* [rows], optional output: the log-probabilities the loss used (0 for rows left out) */
+    float* stats;                             /* [RLGPU_POLICY_STATS], written: sums over the rows that count -- [0] entropy, [1] exp(x) - 1 - x of x = logp - old_logp
+                                               * (the "Mean KL Divergence" of rlgpu_ppo_minibatch), [2] rows with |r - 1| > clip range (on their side), [3] r,
+                                               * [4] exp(d) - 1 - d, [5] rows, [6] the loss, [7] w */
+    void* dlogits; int64_t ld_dlogits;        /* optional output; may be p->logits itself */
+} RlgpuPolicyLoss;
+#define RLGPU_POLICY_STATS 8
+int rlgpu_policy_loss(int device, const RlgpuPolicyRows* p, const RlgpuPolicyLoss* loss, void* workspace, int64_t workspace_bytes, void* hip_stream);
+/* clip_grad_norm over n_tensors dense tensors (host arrays of device pointers, element counts and RLGPU_* types; counts may be 0; up to 2^40 elements each):
+ *   *norm = grad_scale * sqrt(sum over all tensors of g^2)  (device, fp32; summed in 64 bits in a fixed order),
+ *   g *= grad_scale * min(1, max_norm / (*norm + 1e-6))  in place, as rlgpu_clip_adam_step clips.
+ * A norm that is not finite leaves every gradient as it is.  max_norm = +inf with grad_scale = 1 only takes the norm and writes no gradient; any other call
+ * needs tensors that do not overlap.  Workspace as above, rlgpu_clip_grad_workspace(n_tensors) bytes. */
+int64_t rlgpu_clip_grad_workspace(int32_t n_tensors);
+int rlgpu_clip_grad_norm(int device, int32_t n_tensors, void* const* grads, const int64_t* counts, const int32_t* dtypes, float max_norm, float grad_scale,
+                         float* norm, void* workspace, int64_t workspace_bytes, void* hip_stream);
+const char* rlgpu_ops_last_error(void);
+
 /* ---- multi-GPU: one process per GPU, envs sharded across ranks, ONE gradient all-reduce per optimizer step --------
  * Replaces nothing in the reference (it is single-GPU); stands where BASELINE config[2] asks for "RCCL grad all-reduce over xGMI".
  * rlgpu_comm is an RCCL communicator; the data path never leaves the C-ABI (no torch.distributed). */

@@ -46,6 +46,21 @@ class LearnerConfigC(C.Structure):
     ]
 
 
+class PolicyRows(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("ld", C.c_int64), ("mask", C.c_void_p), ("ld_mask", C.c_int64), ("actions", C.c_void_p),
+        ("dtype", C.c_int32), ("rows", C.c_int32), ("n_actions", C.c_int32), ("temperature", C.c_float), ("min_prob", C.c_float),
+    ]
+
+
+class PolicyLossC(C.Structure):
+    _fields_ = [
+        ("old_logp", C.c_void_p), ("adv", C.c_void_p), ("ref_logp", C.c_void_p), ("weights", C.c_void_p),
+        ("clip_low", C.c_float), ("clip_high", C.c_float), ("ent_coef", C.c_float), ("kl_coef", C.c_float), ("scale", C.c_float),
+        ("logp", C.c_void_p), ("stats", C.c_void_p), ("dlogits", C.c_void_p), ("ld_dlogits", C.c_int64),
+    ]
+
+
 _vp = C.c_void_p
 _i = C.c_int
 _f = C.c_float
@@ -174,6 +189,13 @@ SIGNATURES = {
     "rlgpu_lt_write_adam": (_i, [C.c_char_p, _vp, C.c_int, C.c_float, _vp, _vp, C.c_int64]),
     "rlgpu_lt_read_adam": (_i, [C.c_char_p, _vp, C.c_int, _vp, _vp, C.POINTER(C.c_int64)]),
     "rlgpu_lt_last_error": (C.c_char_p, []),
+    "rlgpu_policy_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
+    "rlgpu_action_logp": (_i, [_i, C.POINTER(PolicyRows), _vp, _vp, _vp, C.c_int64, _vp]),
+    "rlgpu_action_logp_backward": (_i, [_i, C.POINTER(PolicyRows), _vp, _vp, _vp, C.c_int64, _vp, C.c_int64, _vp]),
+    "rlgpu_policy_loss": (_i, [_i, C.POINTER(PolicyRows), C.POINTER(PolicyLossC), _vp, C.c_int64, _vp]),
+    "rlgpu_clip_grad_workspace": (C.c_int64, [C.c_int32]),
+    "rlgpu_clip_grad_norm": (_i, [_i, C.c_int32, _vp, _vp, _vp, _f, _f, _vp, _vp, C.c_int64, _vp]),
+    "rlgpu_ops_last_error": (C.c_char_p, []),
 }
 
 _lib = None

@@ -1,0 +1,219 @@
+"""The operators of include/rlgpu.h for a policy network of the caller's own (rlgpu_action_logp, rlgpu_policy_loss, rlgpu_clip_grad_norm): what stands
+around such a network's matrix products in an update, where PPOCore does the same inside the library's own MLPs (the reference's DiscretePolicy and
+PPOLearner: PPO/DiscretePolicy.cpp:44-75, PPO/PPOLearner.cpp:148-215, 273-288).
+
+    r = ops.policy_loss(logits, actions, old_logp, adv, ref_logp, mask, weights, clip_range=0.2, ent_coef=0.005, kl_coef=0.05, scale=1 / rows)
+    logits.backward(r.dlogits)                                  # the rest of the network's backward pass
+    norm = ops.clip_grad_norm([p.grad for p in network.parameters()], 0.5)
+
+Tensors live on one GPU; the work goes to that device's current torch stream, and the outputs are new tensors of it.  Nothing synchronises and nothing is
+kept between calls, so a call may be captured into a graph.  The gradients are explicit calls, not autograd nodes: no call looks at requires_grad.
+Arguments that do not fit raise ValueError before anything runs; an error of the library raises RlgpuError.
+"""
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # RLGPU_F32, RLGPU_BF16, RLGPU_F16
+MIN_PROB = 1e-11                                                    # the floor rlgpu_policy_act puts under a probability (PPO/DiscretePolicy.h:27-32)
+
+# PolicyLoss.stats: sums over the rows that count (not left out)
+STAT_ENTROPY, STAT_KL, STAT_CLIPPED, STAT_RATIO, STAT_REF_KL, STAT_ROWS, STAT_LOSS, STAT_WEIGHT = range(8)
+
+
+class PolicyLoss(NamedTuple):
+    stats: torch.Tensor                 # [8] float32, STAT_*; stats[STAT_LOSS] is the loss
+    logp: torch.Tensor                  # [rows] float32: log-probability of each row's action (0 for rows left out)
+    dlogits: Optional[torch.Tensor]     # [rows, n_actions], the logits' type: d(loss) / d(logits)
+
+
+def _fail(rc):
+    raise _lib.RlgpuError(f"rlgpu error {rc}: {_lib.load().rlgpu_ops_last_error().decode()}")
+
+
+def _vector(name, t, rows, dtype, dev):
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != 1 or t.shape[0] != rows:
+        raise ValueError(f"{name}: a {str(dtype)[6:]} tensor of {rows} rows is needed")
+    if rows > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name}: its rows have to be adjacent")
+    if t.device != dev:
+        raise ValueError(f"{name}: on {t.device}, the logits are on {dev}")
+    return t.data_ptr()
+
+
+def _row_stride(name, t, rows, n):
+    if n > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the actions of a row have to be adjacent")
+    return t.stride(0) if rows > 1 else n
+
+
+def _rows(logits, actions, mask, temperature, min_prob):
+    """The RlgpuPolicyRows of a call, checked."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DTYPES:
+        raise ValueError("logits: a float32, bfloat16 or float16 tensor [rows, n_actions] is needed")
+    rows, n = logits.shape
+    if n < 1 or n > 1 << 28 or rows >= 1 << 31:
+        raise ValueError(f"logits: {rows} rows of {n} actions")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature: {temperature}")
+    if not 0.0 < min_prob < 1.0:
+        raise ValueError(f"min_prob: {min_prob} is not between 0 and 1")
+    dev = logits.device
+    p = _lib.PolicyRows()
+    p.ld = _row_stride("logits", logits, rows, n)
+    if rows > 1 and p.ld < n:
+        raise ValueError("logits: its rows overlap (an expanded tensor)")
+    p.actions = _vector("actions", actions, rows, torch.int32, dev)
+    if mask is not None:
+        if not isinstance(mask, torch.Tensor) or mask.dtype not in (torch.bool, torch.uint8) or mask.shape != logits.shape:
+            raise ValueError(f"mask: a bool or uint8 tensor [{rows}, {n}] is needed (one row for all: mask.expand({rows}, {n}))")
+        if mask.device != dev:
+            raise ValueError(f"mask: on {mask.device}, the logits are on {dev}")
+        p.ld_mask = _row_stride("mask", mask, rows, n)
+        if rows > 1 and 0 < p.ld_mask < n:
+            raise ValueError("mask: its rows overlap")
+        p.mask = mask.data_ptr()
+    if dev.type != "cuda":
+        raise ValueError("logits: the operators run on a GPU (there is no CPU path)")
+    p.logits = logits.data_ptr()
+    p.dtype = _DTYPES[logits.dtype]
+    p.rows, p.n_actions, p.temperature, p.min_prob = rows, n, temperature, min_prob
+    return p, dev
+
+
+def _gradient(out, logits):
+    if out is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.dtype is not logits.dtype or out.device != logits.device:
+        raise ValueError("out: a tensor of the logits' shape, type and device is needed")
+    if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError("out: its rows overlap")
+    return out
+
+
+def _workspace(lib, p, dev):
+    n = lib.rlgpu_policy_workspace(p.dtype, p.rows, p.n_actions)
+    return torch.empty(n, dtype=torch.uint8, device=dev), n
+
+
+def _stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def action_logp(logits, actions, mask=None, *, temperature=1.0, min_prob=MIN_PROB):
+    """(logp, entropy) per row: log max(softmax(logits / temperature)[action], min_prob) and the softmax's entropy over the actions that `mask` (True =
+    allowed) lets through.  actions: int32; one outside [0, n_actions) leaves its row out, as a row in which nothing is allowed is: logp = entropy = 0."""
+    p, dev = _rows(logits, actions, mask, temperature, min_prob)
+    lib = _lib.load()
+    out = torch.empty((2, p.rows), dtype=torch.float32, device=dev)
+    logp, entropy = out[0], out[1]
+    ws, n = _workspace(lib, p, dev)
+    rc = lib.rlgpu_action_logp(dev.index, C.byref(p), logp.data_ptr(), entropy.data_ptr(), ws.data_ptr(), n, _stream(dev))
+    if rc:
+        _fail(rc)
+    return logp, entropy
+
+
+def action_logp_backward(logits, actions, d_logp, d_entropy=None, mask=None, *, temperature=1.0, min_prob=MIN_PROB, out=None):
+    """The gradient of sum(d_logp * logp + d_entropy * entropy) with respect to the logits, in the logits' type.  A logp at the floor passes none, rows left
+    out and actions that are not allowed get 0.  out: where to write it; `logits` itself may be given."""
+    p, dev = _rows(logits, actions, mask, temperature, min_prob)
+    c = _vector("d_logp", d_logp, p.rows, torch.float32, dev)
+    h = _vector("d_entropy", d_entropy, p.rows, torch.float32, dev) if d_entropy is not None else None
+    out = _gradient(out, logits)
+    ld = _row_stride("out", out, p.rows, p.n_actions)
+    lib = _lib.load()
+    ws, n = _workspace(lib, p, dev)
+    rc = lib.rlgpu_action_logp_backward(dev.index, C.byref(p), c, h, out.data_ptr(), ld, ws.data_ptr(), n, _stream(dev))
+    if rc:
+        _fail(rc)
+    return out
+
+
+def policy_loss(logits, actions, old_logp, adv, ref_logp=None, mask=None, weights=None, *, clip_range=0.2, clip_high=None, ent_coef=0.0, kl_coef=0.0,
+                temperature=1.0, min_prob=MIN_PROB, scale=1.0, grad=True, out=None):
+    """scale * sum over rows of w (-min(r A, clip(r, 1 - clip_range, 1 + clip_high) A) + kl_coef (exp(d) - 1 - d) - ent_coef entropy) with
+    r = exp(logp - old_logp), d = ref_logp - logp, and its gradient with respect to the logits, in one pass: a PolicyLoss.  clip_high defaults to
+    clip_range.  A row with weight 0 is left out as in action_logp, and nothing else of it is looked at (padding may hold anything).  grad=False: no gradient.
+    out: where to write the gradient; `logits` itself may be given."""
+    p, dev = _rows(logits, actions, mask, temperature, min_prob)
+    l = _lib.PolicyLossC()
+    l.old_logp = _vector("old_logp", old_logp, p.rows, torch.float32, dev)
+    l.adv = _vector("adv", adv, p.rows, torch.float32, dev)
+    if ref_logp is not None:
+        l.ref_logp = _vector("ref_logp", ref_logp, p.rows, torch.float32, dev)
+    elif kl_coef != 0.0:
+        raise ValueError("kl_coef: needs ref_logp")
+    if weights is not None:
+        l.weights = _vector("weights", weights, p.rows, torch.float32, dev)
+    clip_high = clip_range if clip_high is None else clip_high
+    if not 0.0 <= clip_range < 1.0 or not 0.0 <= clip_high < float("inf"):
+        raise ValueError(f"clip range: {clip_range} below and {clip_high} above 1")
+    l.clip_low, l.clip_high, l.ent_coef, l.kl_coef, l.scale = clip_range, clip_high, ent_coef, kl_coef, scale
+    dlogits = None
+    if grad:
+        dlogits = _gradient(out, logits)
+        l.dlogits, l.ld_dlogits = dlogits.data_ptr(), _row_stride("out", dlogits, p.rows, p.n_actions)
+    elif out is not None:
+        raise ValueError("out: without a gradient there is nothing to write")
+    lib = _lib.load()
+    logp = torch.empty(p.rows, dtype=torch.float32, device=dev)
+    stats = torch.empty(8, dtype=torch.float32, device=dev)
+    l.logp, l.stats = logp.data_ptr(), stats.data_ptr()
+    ws, n = _workspace(lib, p, dev)
+    rc = lib.rlgpu_policy_loss(dev.index, C.byref(p), C.byref(l), ws.data_ptr(), n, _stream(dev))
+    if rc:
+        _fail(rc)
+    return PolicyLoss(stats, logp, dlogits)
+
+
+def clip_grad_norm(grads, max_norm=float("inf"), grad_scale=1.0):
+    """grad_scale * sqrt(sum of the squares of all the tensors' values) as a float32 tensor of one value; the tensors are multiplied in place by
+    grad_scale * min(1, max_norm / (norm + 1e-6)), as PPOCore.clip_adam_step does.  max_norm = inf with grad_scale = 1 only takes the norm.  A norm that is
+    not finite leaves the tensors as they are: look at it before the step.  grads: dense tensors (contiguous, or a permutation of it) of one GPU in float32,
+    bfloat16 or float16, in any mix; None entries (parameters without a gradient) are passed over.  Tensors that overlap are refused when they are written."""
+    grads = [g for g in ([grads] if isinstance(grads, torch.Tensor) else grads) if g is not None]
+    if not grads:
+        raise ValueError("grads: no tensor")
+    if not all(isinstance(g, torch.Tensor) for g in grads):
+        raise ValueError("grads: tensors (or None) are needed")
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm: {max_norm}")
+    if not 0.0 < grad_scale < float("inf"):
+        raise ValueError(f"grad_scale: {grad_scale}")
+    kinds = [_DTYPES.get(g.dtype, -1) for g in grads]
+    if -1 in kinds:
+        raise ValueError(f"grads: {grads[kinds.index(-1)].dtype} is none of float32, bfloat16, float16")
+    for g in grads:
+        if not g.is_contiguous() and not _dense(g):
+            raise ValueError("grads: a tensor is a strided view (its elements have to fill its memory)")
+    dev = grads[0].device
+    if any(g.device != dev for g in grads):
+        raise ValueError("grads: the tensors are on several devices")
+    if dev.type != "cuda":
+        raise ValueError("grads: the operators run on a GPU (there is no CPU path)")
+    lib = _lib.load()
+    n = len(grads)
+    ptrs = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
+    counts = (C.c_int64 * n)(*[g.numel() for g in grads])
+    dtypes = (C.c_int32 * n)(*kinds)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    size = lib.rlgpu_clip_grad_workspace(n)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    rc = lib.rlgpu_clip_grad_norm(dev.index, n, ptrs, counts, dtypes, max_norm, grad_scale, norm.data_ptr(), ws.data_ptr(), size, _stream(dev))
+    if rc:
+        _fail(rc)
+    return norm
+
+
+def _dense(t):
+    """Whether the elements fill the memory they span once: a permutation of a contiguous tensor."""
+    want = 1
+    for size, stride in sorted(((s, st) for s, st in zip(t.shape, t.stride()) if s > 1), key=lambda x: x[1]):
+        if stride != want:
+            return False
+        want *= size
+    return True

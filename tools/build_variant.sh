@@ -12,6 +12,6 @@ mkdir -p _obj/tmp_$NAME
 python3 ../../tools/wwm_lint.py _obj/tmp_$NAME/rlgpu_env-hip-amdgcn-amd-amdhsa-gfx950.s > _obj/rlgpu_env_$NAME.wwm.log || { cat _obj/rlgpu_env_$NAME.wwm.log; exit 1; }
 mv _obj/tmp_$NAME/rlgpu_env.o _obj/rlgpu_env_$NAME.o; rm -rf _obj/tmp_$NAME
 cat _obj/rlgpu_env_$NAME.wwm.log
-/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 _obj/rlgpu_env_$NAME.o _obj/rlgpu_learn.o _obj/rlgpu_comm.o _obj/arena_mesh.o _obj/lt_archive.o \
+/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 _obj/rlgpu_env_$NAME.o _obj/rlgpu_learn.o _obj/rlgpu_ops.o _obj/rlgpu_comm.o _obj/arena_mesh.o _obj/lt_archive.o \
     -o ../librlgpu_$NAME.so -L/opt/rocm/lib -lrccl -lrt -Wl,-rpath,/opt/rocm/lib
 grep -A10 "k_env_collectILi2" _obj/rlgpu_env_$NAME.resource.log | grep -E "VGPRs:|AGPRs|Scratch|Spill|LDS Size" | tr -s ' ' | tr '\n' ';'; echo

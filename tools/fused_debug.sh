@@ -3,7 +3,7 @@
 cd $GRAFT_REPO_ROOT/rlgymppo_cpp_amd/csrc
 mkdir -p /tmp/fzdbg
 /opt/rocm/bin/hipcc -std=c++17 -O3 -fPIC --offload-arch=gfx950 -Wno-unused-value -DFZ_DEBUG $FZ_EXTRA -c rlgpu_learn.hip -o /tmp/fzdbg/rlgpu_learn.o || exit 1
-/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 _obj/rlgpu_env.o /tmp/fzdbg/rlgpu_learn.o _obj/rlgpu_comm.o _obj/arena_mesh.o _obj/lt_archive.o -o /tmp/fzdbg/librlgpu.so -L/opt/rocm/lib -lrccl -lrt -Wl,-rpath,/opt/rocm/lib || exit 1
+/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 _obj/rlgpu_env.o /tmp/fzdbg/rlgpu_learn.o _obj/rlgpu_ops.o _obj/rlgpu_comm.o _obj/arena_mesh.o _obj/lt_archive.o -o /tmp/fzdbg/librlgpu.so -L/opt/rocm/lib -lrccl -lrt -Wl,-rpath,/opt/rocm/lib || exit 1
 cp ../bench_main ../librlgymppo_amd.so /tmp/fzdbg/
 cd $GRAFT_REPO_ROOT
 export TMPDIR=/tmp RLGPU_QUIET=1

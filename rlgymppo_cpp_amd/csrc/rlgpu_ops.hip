@@ -19,10 +19,7 @@
 namespace {
 
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
-constexpr int STATS = RLGPU_POLICY_STATS;
-
-__device__ __forceinline__ float wave_sum(float v) { for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64); return v; }
-__device__ __forceinline__ float wave_max(float v) { for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64)); return v; }
+constexpr int STATS = RLGPU_POLICY_STATS, ROW_BLOCKS = 2048;
 
 template <typename T> struct Lowest;
 template <> struct Lowest<float> { static constexpr float value = -3.4028234663852886e38f; };
@@ -37,7 +34,7 @@ struct RowArgs {
     const float *d_logp, *d_entropy;      // backward
     RlgpuPolicyLoss loss;                 // loss
     void* dlogits; int64_t ldd;           // optional
-    float* row_stats;                     // [rows][STATS]
+    float* row_stats;                     // [workgroups][STATS]: each workgroup's sums over its rows
 };
 enum Mode { LOGP, BACKWARD, LOSS };
 
@@ -48,7 +45,7 @@ __device__ __forceinline__ float exp_minus_1_minus(float x) {
     return expf(x) - 1.f - x;
 }
 
-// one row of the loss: d loss / d logp and d loss / d entropy, and the row's part of the statistics
+// one row of the loss: d loss / d logp and d loss / d entropy, and the row's part of the statistics (added to st)
 __device__ void loss_row(const RowArgs& g, int row, float w, float logp, float H, bool floored, float& c, float& h, float (&st)[STATS]) {
     const RlgpuPolicyLoss& l = g.loss;
     const float x = logp - l.old_logp[row], adv = l.adv[row];
@@ -66,78 +63,232 @@ __device__ void loss_row(const RowArgs& g, int row, float w, float logp, float H
     value -= l.ent_coef * H;
     c = floored ? 0.f : c * w * l.scale;
     h = -l.ent_coef * w * l.scale;
-    st[0] = H; st[1] = exp_minus_1_minus(x); st[2] = (r < 1.f - l.clip_low || r > 1.f + l.clip_high) ? 1.f : 0.f; st[3] = r;
-    st[4] = ref; st[5] = 1.f; st[6] = value * w * l.scale; st[7] = w;
+    st[0] += H; st[1] += exp_minus_1_minus(x); st[2] += (r < 1.f - l.clip_low || r > 1.f + l.clip_high) ? 1.f : 0.f; st[3] += r;
+    st[4] += ref; st[5] += 1.f; st[6] += value * w * l.scale; st[7] += w;
 }
 
-// One workgroup of 256 threads a row, three readings of it.
-template <typename T, Mode MODE>
-__global__ void __launch_bounds__(256) k_rows(RowArgs g) {
-    __shared__ float red[3][4];
-    const int row = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, A = g.p.n_actions;
-    const T* x = (const T*)g.p.logits + (int64_t)row * g.p.ld;
-    const uint8_t* mask = g.p.mask ? g.p.mask + (int64_t)row * g.p.ld_mask : nullptr;
-    T* dx = (T*)g.dlogits + (int64_t)row * g.ldd;
-    auto at = [&](int i) -> float { return mask && !mask[i] ? -INFINITY : (float)x[i]; };
-    const int a = g.p.actions[row];
-    const float w = MODE == LOSS && g.loss.weights ? g.loss.weights[row] : 1.f;
-    bool on = a >= 0 && a < A && w != 0.f;
-    float logp = 0.f, H = 0.f, c = 0.f, h = 0.f, mc = 0.f, L = 0.f, lpa = 0.f;
+// ---- 16 bytes of a row --------------------------------------------------------------------------------------------------------------------------------
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;      // a row starts wherever its stride puts it: global memory takes 16-byte accesses at any address
+typedef uint64_t __attribute__((aligned(1))) u64_any;
+typedef uint32_t __attribute__((aligned(1))) u32_any;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
+using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
+
+template <typename T> struct Pack;                        // N values of T in 16 bytes
+template <> struct Pack<float> {
+    static constexpr int N = 4; static constexpr uint32_t NEG_INF = 0xff800000u;
+    static __device__ __forceinline__ float get(u32x4 v, int j) { const uint32_t w = v[j]; return __builtin_bit_cast(float, w); }   // (of v[j] itself the builtin takes element 0)
+    static __device__ __forceinline__ u32x4 put(const float (&d)[4]) { u32x4 v; for (int j = 0; j < 4; j++) v[j] = __builtin_bit_cast(uint32_t, d[j]); return v; }
+    using Bytes = uint32_t;                               // the mask of N values
+    static __device__ __forceinline__ Bytes bytes(const uint8_t* m) { return *(const u32_any*)m; }
+    static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) {
+        for (int j = 0; j < 4; j++) v[j] = (b >> (8 * j)) & 0xff ? v[j] : NEG_INF;
+        return v;
+    }
+};
+template <typename T, typename T2> struct Pack16 {
+    static constexpr int N = 8;
+    using Bytes = uint64_t;
+    static __device__ __forceinline__ Bytes bytes(const uint8_t* m) { return *(const u64_any*)m; }
+    static __device__ __forceinline__ u32x4 put(const float (&d)[8]) {
+        u32x4 v;
+        for (int j = 0; j < 4; j++) v[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{d[2 * j], d[2 * j + 1]}), T2));
+        return v;
+    }
+    static __device__ __forceinline__ u32x4 forbid16(u32x4 v, Bytes b, uint32_t neg_inf) {
+        for (int j = 0; j < 4; j++) {
+            const uint32_t w = (uint32_t)(b >> (16 * j));
+            v[j] = ((w & 0xff) ? v[j] & 0xffffu : neg_inf) | ((w & 0xff00) ? v[j] & 0xffff0000u : neg_inf << 16);
+        }
+        return v;
+    }
+};
+template <> struct Pack<__bf16> : Pack16<__bf16, bf16x2> {
+    static constexpr uint32_t NEG_INF = 0xff80ff80u;
+    static __device__ __forceinline__ float get(u32x4 v, int j) { const uint32_t w = v[j >> 1]; return __builtin_bit_cast(float, j & 1 ? w & 0xffff0000u : w << 16); }
+    static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xff80u); }
+};
+template <> struct Pack<_Float16> : Pack16<_Float16, f16x2> {
+    static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+    static __device__ __forceinline__ float get(u32x4 v, int j) { return (float)__builtin_bit_cast(f16x2, (uint32_t)v[j >> 1])[j & 1]; }
+    static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xfc00u); }
+};
+
+// The larger of three.  (fmaxf would first quiet each operand, an instruction a value; a NaN that is dropped here still makes the row's sum NaN.)
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c)); return r; }
+
+// Between two pieces of a pass, all that it sums being here by then.  Left alone, the compiler unpacks every piece first and adds later, or keeps the 32-bit
+// values of one pass for the next (219 registers where 32 hold a row in 16 bits, and spills in the largest).
+__device__ __forceinline__ void piece_done(u32x4& v, float& m) { asm("" : "+v"(v), "+v"(m)); __builtin_amdgcn_sched_barrier(0); }
+__device__ __forceinline__ void piece_done(u32x4& v, float (&s)[4], float (&w)[4]) {
+    asm("" : "+v"(v), "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]), "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// ---- sums and maxima over the G lanes of a row; G = 16 stays in a DPP row, more than 64 goes through LDS (`red`: one float a wavefront) ----------------------
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+}
+struct Sum { static __device__ __forceinline__ float of(float a, float b) { return a + b; } };
+struct Max { static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); } };
+template <int N, typename OP> __device__ __forceinline__ float lanes(float v) {       // over aligned groups of N lanes, every lane gets the result
+    v = OP::of(v, dpp<0xB1>(v));                          // quad_perm 1 0 3 2
+    if (N > 2) v = OP::of(v, dpp<0x4E>(v));               // quad_perm 2 3 0 1
+    if (N > 4) v = OP::of(v, dpp<0x141>(v));              // row_half_mirror
+    if (N > 8) v = OP::of(v, dpp<0x140>(v));              // row_mirror
+    if (N > 16) { v = OP::of(v, __shfl_xor(v, 16, 64)); v = OP::of(v, __shfl_xor(v, 32, 64)); }
+    return v;
+}
+template <int G, typename OP> __device__ __forceinline__ void put_wave(float v, float* red) { v = lanes<64, OP>(v); if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v; }
+template <int G, typename OP> __device__ __forceinline__ float get_waves(const float* red) { constexpr int W = G / 64; return lanes<W, OP>(red[threadIdx.x & (W - 1)]); }
+
+// G lanes take a row and hold it in registers, NV times 16 bytes each, from its one reading to the writing of the gradient.  What is over after the whole
+// 16-byte pieces (fewer than G values) goes to the first lanes, one value each.  MORE: the row may be longer than the registers; the pieces beyond are read
+// twice, once into a running maximum and sum, and once for the gradient.
+template <typename T, int G, int NV, Mode MODE, bool MORE>
+__global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
+    using P = Pack<T>;
+    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64;
+    __shared__ float red[3][W], sums[RPB][STATS];
+    const int lane = G <= 64 ? threadIdx.x % G : threadIdx.x, sub = G <= 64 ? threadIdx.x / G : 0;
+    const int A = g.p.n_actions, whole = A / N, rest = A - whole * N;
     float st[STATS] = {};
-    if (on) {
-        const float xa = at(a);
-        float m = -INFINITY;
-        for (int i = tid; i < A; i += 256) m = fmaxf(m, at(i));
-        m = wave_max(m);
-        if ((tid & 63) == 0) red[0][wave] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-        // a row without an allowed action (or one of NaN alone: fmaxf passes over NaN) is summed against 0: it gives 0 or NaN
-        const bool live = m > Lowest<T>::value && fabsf(m * g.k) < 3e38f;
-        mc = live ? m * g.k : 0.f;
-        float S = 0.f, W = 0.f;
-        for (int i = tid; i < A; i += 256) {
-            const float t = fmaf(at(i), g.k, -mc), e = exp2f(t);
-            S += e; W += e * fmaxf(t, -1e30f);
-        }
-        S = wave_sum(S); W = wave_sum(W);
-        if ((tid & 63) == 0) { red[1][wave] = S; red[2][wave] = W; }
-        __syncthreads();
-        S = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]); W = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
-        if (!live) { on = S != 0.f; S = NAN; }
+    for (int row = blockIdx.x * RPB + sub; row < g.p.rows; row += gridDim.x * RPB) {
+        const T* x = (const T*)g.p.logits + (int64_t)row * g.p.ld;
+        const uint8_t* mask = g.p.mask ? g.p.mask + (int64_t)row * g.p.ld_mask : nullptr;
+        T* dx = (T*)g.dlogits + (int64_t)row * g.ldd;
+        const int a = g.p.actions[row];
+        const float w = MODE == LOSS && g.loss.weights ? g.loss.weights[row] : 1.f;
+        bool on = a >= 0 && a < A && w != 0.f;
+        auto one = [&](int i) -> float { return mask && !mask[i] ? -INFINITY : (float)x[i]; };
+        auto piece = [&](int c) -> u32x4 { u32x4 v = *(const u32x4_any*)(x + c * N); if (mask) v = P::forbid(v, P::bytes(mask + c * N)); return v; };
+        float logp = 0.f, H = 0.f, c = 0.f, h = 0.f, mc = 0.f, L = 0.f, lpa = 0.f;
+        u32x4 v[NV]; float xt = -INFINITY;
         if (on) {
-            L = log2f(S);
-            H = LN2 * (L - W / S);
-            lpa = LN2 * (fmaf(xa, g.k, -mc) - L);
-            H = H < 0.f ? 0.f : H; lpa = lpa > 0.f ? 0.f : lpa;          // (the rounding of mc can leave either an ulp of t off; a NaN stays)
-            const bool floored = lpa < g.log_floor;
-            logp = floored ? g.log_floor : lpa;
-            if (MODE == BACKWARD) { c = floored ? 0.f : g.d_logp[row]; h = g.d_entropy ? g.d_entropy[row] : 0.f; }
-            if (MODE == LOSS) loss_row(g, row, w, logp, H, floored, c, h, st);
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                v[i] = u32x4{P::NEG_INF, P::NEG_INF, P::NEG_INF, P::NEG_INF};
+                if (lane + i * G < whole) v[i] = *(const u32x4_any*)(x + (lane + i * G) * N);
+            }
+            if (mask) {
+                typename P::Bytes b[NV];
+#pragma unroll
+                for (int i = 0; i < NV; i++) { b[i] = 0; if (lane + i * G < whole) b[i] = P::bytes(mask + (lane + i * G) * N); }
+#pragma unroll
+                for (int i = 0; i < NV; i++) { v[i] = P::forbid(v[i], b[i]); __builtin_amdgcn_sched_barrier(0); }
+            }
+            if (lane < rest) xt = one(whole * N + lane);
+            const float xa = one(a);
+            float m = xt, S = 0.f, Wt = 0.f, more_mc = 0.f;
+            if (MORE) {
+                m = -INFINITY;
+                for (int k = lane + NV * G; k < whole; k += G) {
+                    const u32x4 q = piece(k);
+                    float top = P::get(q, 0);
+#pragma unroll
+                    for (int j = 1; j < N; j++) top = fmaxf(top, P::get(q, j));
+                    if (top > m) {                        // (what is summed so far moves to the new maximum: S 2^(old - new), and W with each t)
+                        const float to = fabsf(top * g.k) < 3e38f ? top * g.k : 0.f, by = more_mc - to, f = S > 0.f ? __builtin_amdgcn_exp2f(by) : 0.f;
+                        Wt = f * (Wt + S * by); S *= f; m = top; more_mc = to;
+                    }
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        const float t = fmaf(P::get(q, j), g.k, -more_mc), e = __builtin_amdgcn_exp2f(t);
+                        S += e; Wt = fmaf(e, fmaxf(t, -1e30f), Wt);
+                    }
+                }
+                m = fmaxf(m, xt);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+#pragma unroll
+                for (int j = 0; j < N; j += 2) m = max3(m, P::get(v[i], j), P::get(v[i], j + 1));
+                piece_done(v[i], m);
+            }
+            if (G <= 64) m = lanes<G, Max>(m);
+            else { put_wave<G, Max>(m, red[0]); __syncthreads(); m = get_waves<G, Max>(red[0]); }
+            // a row without an allowed action (or one of NaN alone: the maximum passes over NaN) is summed against 0: it gives 0 or NaN
+            const bool live = m > Lowest<T>::value && fabsf(m * g.k) < 3e38f;
+            mc = live ? m * g.k : 0.f;
+            if (MORE && S != 0.f) { const float by = more_mc - mc, f = __builtin_amdgcn_exp2f(by); Wt = f * (Wt + S * by); S *= f; }
+            float S4[4] = {S, 0.f, 0.f, 0.f}, W4[4] = {Wt, 0.f, 0.f, 0.f};
+            auto add = [&](float xv, int j) {
+                const float t = fmaf(xv, g.k, -mc), e = __builtin_amdgcn_exp2f(t);
+                S4[j & 3] += e; W4[j & 3] = fmaf(e, fmaxf(t, -1e30f), W4[j & 3]);        // (e = 0 where t is -inf)
+            };
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+#pragma unroll
+                for (int j = 0; j < N; j++) add(P::get(v[i], j), j);
+                piece_done(v[i], S4, W4);
+            }
+            add(xt, 3);
+            S = (S4[0] + S4[1]) + (S4[2] + S4[3]); Wt = (W4[0] + W4[1]) + (W4[2] + W4[3]);
+            if (G <= 64) { S = lanes<G, Sum>(S); Wt = lanes<G, Sum>(Wt); }
+            else {
+                put_wave<G, Sum>(S, red[1]); put_wave<G, Sum>(Wt, red[2]);
+                __syncthreads();
+                S = get_waves<G, Sum>(red[1]); Wt = get_waves<G, Sum>(red[2]);
+            }
+            if (!live) { on = S != 0.f; S = NAN; }
+            if (on) {
+                L = log2f(S);
+                H = LN2 * (L - Wt / S);
+                lpa = LN2 * (fmaf(xa, g.k, -mc) - L);
+                H = H < 0.f ? 0.f : H;                                   // (the rounding of mc can leave either an ulp of t off; a NaN stays)
+                lpa = lpa > 0.f ? 0.f : (lpa < -1e30f ? -1e30f : lpa);   // (-inf: below every floor, and 0 times it is wanted below)
+                const bool floored = lpa < g.log_floor;
+                logp = floored ? g.log_floor : lpa;
+                if (MODE == BACKWARD) { c = floored ? 0.f : g.d_logp[row]; h = g.d_entropy ? g.d_entropy[row] : 0.f; }
+                if (MODE == LOSS) loss_row(g, row, w, logp, H, floored, c, h, st);
+            }
         }
-    }
-    if (tid == 0) {
-        if (g.logp) g.logp[row] = logp;
-        if (g.entropy) g.entropy[row] = H;
-    }
-    if (MODE == LOSS && tid < STATS) g.row_stats[(int64_t)row * STATS + tid] = st[tid];
-    if (MODE == LOGP || !g.dlogits) return;
-    for (int i = tid; i < A; i += 256) {
-        float d = 0.f;
-        if (on) {
-            const float t = fmaxf(fmaf(at(i), g.k, -mc), -1e30f), s = exp2f(t - L);
-            d = -s * (c + h * (LN2 * (t - L) + H)) + (i == a ? c : 0.f);
+        if (lane == 0) {
+            if (g.logp) g.logp[row] = logp;
+            if (g.entropy) g.entropy[row] = H;
         }
-        dx[i] = (T)(d * g.inv_t);
+        if (MODE == LOGP || !g.dlogits) continue;
+        if (!on) {
+            for (int k = lane; k < whole; k += G) *(u32x4_any*)(dx + k * N) = u32x4{0, 0, 0, 0};
+            if (lane < rest) dx[whole * N + lane] = (T)0.f;
+            continue;
+        }
+        // e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i); the action's own c / T comes in a store of its own behind it
+        const float inv = g.inv_t * __builtin_amdgcn_exp2f(-L), p1 = -h * LN2 * inv, p0 = -(c + h * (H - LN2 * L)) * inv;
+        auto grad = [&](float xv) -> float { const float t = fmaxf(fmaf(xv, g.k, -mc), -1e30f); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); };
+        auto store = [&](int k, u32x4 q) {
+            float d[N];
+#pragma unroll
+            for (int j = 0; j < N; j++) d[j] = grad(P::get(q, j));
+            *(u32x4_any*)(dx + k * N) = P::put(d);
+        };
+#pragma unroll
+        for (int i = 0; i < NV; i++) { if (lane + i * G < whole) store(lane + i * G, v[i]); __builtin_amdgcn_sched_barrier(0); }
+        if (MORE) for (int k = lane + NV * G; k < whole; k += G) store(k, piece(k));
+        if (lane < rest) dx[whole * N + lane] = (T)grad(xt);
+        const int ka = a / N;
+        if (lane == (ka < whole ? ka % G : a - whole * N))
+            dx[a] = (T)((-c * expm1f(lpa) - h * expf(lpa) * (lpa + H)) * g.inv_t);       // c (1 - s) - h s (log s + H): its lane wrote the 16 bytes around it
+    }
+    if (MODE != LOSS) return;
+    if (lane == 0) for (int k = 0; k < STATS; k++) sums[sub][k] = st[k];
+    __syncthreads();
+    if (threadIdx.x < STATS) {
+        float s = sums[0][threadIdx.x];
+        for (int k = 1; k < RPB; k++) s += sums[k][threadIdx.x];
+        g.row_stats[(int64_t)blockIdx.x * STATS + threadIdx.x] = s;
     }
 }
 
-// the rows' statistics in a fixed order: 64 slices of rows, then the slices, in 64 bits
-__global__ void __launch_bounds__(512) k_row_stats(const float* part, int64_t n, float* stats) {
+// the workgroups' statistics in a fixed order: 64 slices of them, then the slices, in 64 bits
+__global__ void __launch_bounds__(512) k_row_stats(const float* part, int n, float* stats) {
     __shared__ double red[512];
     const int k = threadIdx.x & 7;
     double s = 0;
-    for (int64_t i = threadIdx.x >> 3; i < n; i += 64) s += (double)part[i * STATS + k];
+    for (int i = threadIdx.x >> 3; i < n; i += 64) s += (double)part[i * STATS + k];
     red[threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.x < STATS) {
@@ -235,7 +386,7 @@ struct OnDevice {
 int64_t size_of(int dtype) { return dtype == RLGPU_F32 ? 4 : (dtype == RLGPU_BF16 || dtype == RLGPU_F16 ? 2 : 0); }
 bool misaligned(const void* p, int64_t to) { return (uintptr_t)p % (uintptr_t)to != 0; }
 
-int64_t workspace_bytes_for(int rows) { return std::max<int64_t>(16, (int64_t)rows * STATS * 4); }
+int64_t workspace_bytes_for(int rows) { return std::max<int64_t>(16, (int64_t)std::min(rows, ROW_BLOCKS) * STATS * 4); }
 
 int check_rows(const char* who, const RlgpuPolicyRows* p, const void* workspace, int64_t bytes) {
     if (!p) return fail(RLGPU_ERR_ARG, "%s: no rows", who);
@@ -274,14 +425,30 @@ RowArgs row_args(const RlgpuPolicyRows* p) {
     g.inv_t = 1.f / p->temperature; g.k = (float)(1.4426950408889634 / (double)p->temperature); g.log_floor = (float)std::log((double)p->min_prob);
     return g;
 }
-template <Mode MODE> int launch_rows(const RowArgs& g, hipStream_t s) {
-    if (g.p.rows == 0) return RLGPU_OK;
-    const dim3 grid(g.p.rows), block(256);
-    if (g.p.dtype == RLGPU_F32) hipLaunchKernelGGL((k_rows<float, MODE>), grid, block, 0, s, g);
-    else if (g.p.dtype == RLGPU_BF16) hipLaunchKernelGGL((k_rows<__bf16, MODE>), grid, block, 0, s, g);
-    else hipLaunchKernelGGL((k_rows<_Float16, MODE>), grid, block, 0, s, g);
-    OCHK(hipGetLastError());
+// Lanes and 16-byte pieces a row: the smallest set of registers that holds it.  Workgroups: as many as the device keeps at once, each taking rows in turn.
+template <typename T, Mode MODE> int launch_rows_of(const RowArgs& g, hipStream_t s, int& blocks) {
+    const int whole = g.p.n_actions / Pack<T>::N;
+#define ROWS(G, NV, MORE)                                                                                                        \
+    do {                                                                                                                         \
+        if (MORE || whole <= (G) * (NV)) {                                                                                       \
+            const int rpb = (G) <= 64 ? 256 / (G) : 1;                                                                           \
+            blocks = std::min(ROW_BLOCKS, (g.p.rows + rpb - 1) / rpb);                                                           \
+            hipLaunchKernelGGL((k_rows<T, G, NV, MODE, MORE>), dim3(blocks), dim3((G) <= 64 ? 256 : (G)), 0, s, g);              \
+            OCHK(hipGetLastError());                                                                                             \
+            return RLGPU_OK;                                                                                                     \
+        }                                                                                                                        \
+    } while (0)
+    ROWS(16, 1, false); ROWS(16, 2, false); ROWS(64, 1, false); ROWS(64, 2, false); ROWS(64, 4, false);
+    ROWS(256, 2, false); ROWS(256, 4, false); ROWS(256, 8, false); ROWS(1024, 4, false); ROWS(1024, 8, false); ROWS(1024, 16, true);
+#undef ROWS
     return RLGPU_OK;
+}
+template <Mode MODE> int launch_rows(const RowArgs& g, hipStream_t s, int& blocks) {
+    blocks = 0;
+    if (g.p.rows == 0) return RLGPU_OK;
+    if (g.p.dtype == RLGPU_F32) return launch_rows_of<float, MODE>(g, s, blocks);
+    if (g.p.dtype == RLGPU_BF16) return launch_rows_of<__bf16, MODE>(g, s, blocks);
+    return launch_rows_of<_Float16, MODE>(g, s, blocks);
 }
 
 int clip_batches(int n) { return std::max(1, (n + TENSORS - 1) / TENSORS); }
@@ -305,7 +472,8 @@ int rlgpu_action_logp(int device, const RlgpuPolicyRows* p, float* logp, float* 
     const OnDevice on(device); OCHK(on.err);
     RowArgs g = row_args(p);
     g.logp = logp; g.entropy = entropy;
-    return launch_rows<LOGP>(g, (hipStream_t)stream);
+    int blocks;
+    return launch_rows<LOGP>(g, (hipStream_t)stream, blocks);
 }
 
 int rlgpu_action_logp_backward(int device, const RlgpuPolicyRows* p, const float* d_logp, const float* d_entropy, void* dlogits, int64_t ld_dlogits,
@@ -318,7 +486,8 @@ int rlgpu_action_logp_backward(int device, const RlgpuPolicyRows* p, const float
     const OnDevice on(device); OCHK(on.err);
     RowArgs g = row_args(p);
     g.d_logp = d_logp; g.d_entropy = d_entropy; g.dlogits = dlogits; g.ldd = ld_dlogits;
-    return launch_rows<BACKWARD>(g, (hipStream_t)stream);
+    int blocks;
+    return launch_rows<BACKWARD>(g, (hipStream_t)stream, blocks);
 }
 
 int rlgpu_policy_loss(int device, const RlgpuPolicyRows* p, const RlgpuPolicyLoss* l, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -338,8 +507,9 @@ int rlgpu_policy_loss(int device, const RlgpuPolicyRows* p, const RlgpuPolicyLos
     const OnDevice on(device); OCHK(on.err);
     RowArgs g = row_args(p);
     g.loss = *l; g.logp = l->logp; g.dlogits = l->dlogits; g.ldd = l->ld_dlogits; g.row_stats = (float*)workspace;
-    if (int rc = launch_rows<LOSS>(g, (hipStream_t)stream)) return rc;
-    hipLaunchKernelGGL(k_row_stats, dim3(1), dim3(512), 0, (hipStream_t)stream, (const float*)workspace, (int64_t)p->rows, l->stats);
+    int blocks;
+    if (int rc = launch_rows<LOSS>(g, (hipStream_t)stream, blocks)) return rc;
+    hipLaunchKernelGGL(k_row_stats, dim3(1), dim3(512), 0, (hipStream_t)stream, (const float*)workspace, blocks, l->stats);
     OCHK(hipGetLastError());
     return RLGPU_OK;
 }

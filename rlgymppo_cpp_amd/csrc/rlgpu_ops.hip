@@ -2,7 +2,7 @@
 // policy loss with a KL term, both with their gradients, and the gradient norm over many tensors with the clip.
 //
 // The mathematics of a row of logits x (temperature T, k = log2(e) / T, all exponentials in base 2):
-//   t_i = k (x_i - max x) <= 0, e_i = 2^t_i, S = sum e_i, W = sum e_i t_i, L = log2 S
+//   t_i = k x_i - m for an m near k max x, e_i = 2^t_i, S = sum e_i, W = sum e_i t_i, L = log2 S
 //   log s_i = ln2 (t_i - L), entropy H = -sum s_i log s_i = ln2 (L - W / S)
 //   d(c logp + h H) / dx_i = (1/T) [c (1{i = a} - s_i) - h s_i (log s_i + H)]
 // so one reading of the row gives everything a row needs (S and W), and a second one, from wherever the row still is, the gradient.
@@ -11,6 +11,8 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstring>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -19,17 +21,14 @@
 namespace {
 
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
-constexpr int STATS = RLGPU_POLICY_STATS, ROW_BLOCKS = 2048;
-
-template <typename T> struct Lowest;
-template <> struct Lowest<float> { static constexpr float value = -3.4028234663852886e38f; };
-template <> struct Lowest<__bf16> { static constexpr float value = -3.3895313892515355e38f; };
-template <> struct Lowest<_Float16> { static constexpr float value = -65504.f; };
+constexpr int STATS = RLGPU_POLICY_STATS, ROW_BLOCKS = 2048, BLOCKS_OF_1024 = 256;
 
 // what a launch over rows takes; mode decides which of the outputs are there
 struct RowArgs {
     RlgpuPolicyRows p;
     float k, inv_t, log_floor;            // log2(e) / T, 1 / T, log(min_prob)
+    float no_m;                           // a row whose m is no larger has nothing allowed
+    unsigned turn;
     float *logp, *entropy;                // optional
     const float *d_logp, *d_entropy;      // backward
     RlgpuPolicyLoss loss;                 // loss
@@ -45,7 +44,7 @@ __device__ __forceinline__ float exp_minus_1_minus(float x) {
     return expf(x) - 1.f - x;
 }
 
-// one row of the loss: d loss / d logp and d loss / d entropy, and the row's part of the statistics (added to st)
+// one row of the loss: d loss / d logp and d loss / d entropy, and the row's part of the statistics
 __device__ void loss_row(const RowArgs& g, int row, float w, float logp, float H, bool floored, float& c, float& h, float (&st)[STATS]) {
     const RlgpuPolicyLoss& l = g.loss;
     const float x = logp - l.old_logp[row], adv = l.adv[row];
@@ -63,8 +62,8 @@ __device__ void loss_row(const RowArgs& g, int row, float w, float logp, float H
     value -= l.ent_coef * H;
     c = floored ? 0.f : c * w * l.scale;
     h = -l.ent_coef * w * l.scale;
-    st[0] += H; st[1] += exp_minus_1_minus(x); st[2] += (r < 1.f - l.clip_low || r > 1.f + l.clip_high) ? 1.f : 0.f; st[3] += r;
-    st[4] += ref; st[5] += 1.f; st[6] += value * w * l.scale; st[7] += w;
+    st[0] = H; st[1] = exp_minus_1_minus(x); st[2] = (r < 1.f - l.clip_low || r > 1.f + l.clip_high) ? 1.f : 0.f; st[3] = r;
+    st[4] = ref; st[5] = 1.f; st[6] = value * w * l.scale; st[7] = w;
 }
 
 // ---- 16 bytes of a row --------------------------------------------------------------------------------------------------------------------------------
@@ -76,15 +75,17 @@ using f32x2 = __attribute__((ext_vector_type(2))) float;
 using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 
-template <typename T> struct Pack;                        // N values of T in 16 bytes
+// N values of T in 16 bytes.  FILL, an action that is not allowed and places behind a row's end: low enough to be 0 in any sum, finite (an e t of 0 times -inf
+// would be NaN), and a row whose largest logit is no larger has nothing allowed (-9.97e36; float16: its lowest value, -65504).
+template <typename T> struct Pack;
 template <> struct Pack<float> {
-    static constexpr int N = 4; static constexpr uint32_t NEG_INF = 0xff800000u;
+    static constexpr int N = 4; static constexpr uint32_t FILL = 0xfcf00000u;
     static __device__ __forceinline__ float get(u32x4 v, int j) { const uint32_t w = v[j]; return __builtin_bit_cast(float, w); }   // (of v[j] itself the builtin takes element 0)
     static __device__ __forceinline__ u32x4 put(const float (&d)[4]) { u32x4 v; for (int j = 0; j < 4; j++) v[j] = __builtin_bit_cast(uint32_t, d[j]); return v; }
     using Bytes = uint32_t;                               // the mask of N values
     static __device__ __forceinline__ Bytes bytes(const uint8_t* m) { return *(const u32_any*)m; }
     static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) {
-        for (int j = 0; j < 4; j++) v[j] = (b >> (8 * j)) & 0xff ? v[j] : NEG_INF;
+        for (int j = 0; j < 4; j++) v[j] = (b >> (8 * j)) & 0xff ? v[j] : FILL;
         return v;
     }
 };
@@ -97,35 +98,65 @@ template <typename T, typename T2> struct Pack16 {
         for (int j = 0; j < 4; j++) v[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{d[2 * j], d[2 * j + 1]}), T2));
         return v;
     }
-    static __device__ __forceinline__ u32x4 forbid16(u32x4 v, Bytes b, uint32_t neg_inf) {
+    static __device__ __forceinline__ u32x4 forbid16(u32x4 v, Bytes b, uint32_t fill) {
         for (int j = 0; j < 4; j++) {
             const uint32_t w = (uint32_t)(b >> (16 * j));
-            v[j] = ((w & 0xff) ? v[j] & 0xffffu : neg_inf) | ((w & 0xff00) ? v[j] & 0xffff0000u : neg_inf << 16);
+            v[j] = ((w & 0xff) ? v[j] & 0xffffu : fill) | ((w & 0xff00) ? v[j] & 0xffff0000u : fill << 16);
         }
         return v;
     }
 };
 template <> struct Pack<__bf16> : Pack16<__bf16, bf16x2> {
-    static constexpr uint32_t NEG_INF = 0xff80ff80u;
+    static constexpr uint32_t FILL = 0xfcf0fcf0u;
     static __device__ __forceinline__ float get(u32x4 v, int j) { const uint32_t w = v[j >> 1]; return __builtin_bit_cast(float, j & 1 ? w & 0xffff0000u : w << 16); }
-    static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xff80u); }
+    static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xfcf0u); }
 };
 template <> struct Pack<_Float16> : Pack16<_Float16, f16x2> {
-    static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+    static constexpr uint32_t FILL = 0xfbfffbffu;
     static __device__ __forceinline__ float get(u32x4 v, int j) { return (float)__builtin_bit_cast(f16x2, (uint32_t)v[j >> 1])[j & 1]; }
-    static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xfc00u); }
+    static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xfbffu); }
 };
 
 // The larger of three.  (fmaxf would first quiet each operand, an instruction a value; a NaN that is dropped here still makes the row's sum NaN.)
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c)); return r; }
 
-// Between two pieces of a pass, all that it sums being here by then.  Left alone, the compiler unpacks every piece first and adds later, or keeps the 32-bit
-// values of one pass for the next (219 registers where 32 hold a row in 16 bits, and spills in the largest).
-__device__ __forceinline__ void piece_done(u32x4& v, float& m) { asm("" : "+v"(v), "+v"(m)); __builtin_amdgcn_sched_barrier(0); }
-__device__ __forceinline__ void piece_done(u32x4& v, float (&s)[4], float (&w)[4]) {
-    asm("" : "+v"(v), "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]), "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
-    __builtin_amdgcn_sched_barrier(0);
-}
+// Between two pieces of a row.  Left alone, the scheduler unpacks every piece first and adds later, as the sums are one long chain, or keeps the 32-bit values of
+// one pass for the next (219 registers where 32 hold a row in 16 bits, and spills in the largest).
+__device__ __forceinline__ void piece_done() { __builtin_amdgcn_sched_barrier(0); }
+
+// What a lane has of S and W.  `m` is the exponent (k x) that its sums are taken against: not the maximum, but within SLACK of it, so that it hardly ever moves
+// after the first piece and a row is summed in one pass, piece by piece as it arrives.
+constexpr float SLACK = 8.f, NO_M = -1e38f;
+struct RowSum {
+    float m, s[2], w[2];
+    __device__ __forceinline__ void clear() { m = NO_M; s[0] = s[1] = w[0] = w[1] = 0.f; }
+    // `top`: the largest x of what comes next
+    __device__ __forceinline__ void reach(float top, float k) {
+        const float to = top * k;
+        if (to > m + SLACK) {
+            const bool fits = to < 3e38f;
+            const float by = m - (fits ? to : 0.f), f = __builtin_amdgcn_exp2f(by);
+            for (int j = 0; j < 2; j++) { w[j] = f * fmaf(s[j], by, w[j]); s[j] *= f; }
+            m = fits ? to : 0.f;
+            if (!fits) s[0] = NAN;                        // +inf among the logits
+        }
+    }
+    // CAREFUL: some t may be -inf, and 0 times it is to be 0
+    template <bool CAREFUL> __device__ __forceinline__ void add(float x, float k, int j) {
+        const float t = fmaf(x, k, -m), e = __builtin_amdgcn_exp2f(t);
+        s[j] += e; w[j] = fmaf(e, CAREFUL ? fmaxf(t, -1e30f) : t, w[j]);
+    }
+    template <bool CAREFUL, typename P> __device__ __forceinline__ void piece(u32x4& v, float k) {
+        float top = max3(P::get(v, 0), P::get(v, 1), P::get(v, 2));
+#pragma unroll
+        for (int j = 3; j + 1 < P::N; j += 2) top = max3(top, P::get(v, j), P::get(v, j + 1));
+        reach(max3(top, P::get(v, P::N - 1), P::get(v, P::N - 1)), k);
+#pragma unroll
+        for (int j = 0; j < P::N; j++) add<CAREFUL>(P::get(v, j), k, j & 1);
+        asm("" : "+v"(v), "+v"(s[0]), "+v"(s[1]), "+v"(w[0]), "+v"(w[1]));
+        piece_done();
+    }
+};
 
 // ---- sums and maxima over the G lanes of a row; G = 16 stays in a DPP row, more than 64 goes through LDS (`red`: one float a wavefront) ----------------------
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
@@ -146,139 +177,169 @@ template <int G, typename OP> __device__ __forceinline__ void put_wave(float v, 
 template <int G, typename OP> __device__ __forceinline__ float get_waves(const float* red) { constexpr int W = G / 64; return lanes<W, OP>(red[threadIdx.x & (W - 1)]); }
 
 // G lanes take a row and hold it in registers, NV times 16 bytes each, from its one reading to the writing of the gradient.  What is over after the whole
-// 16-byte pieces (fewer than G values) goes to the first lanes, one value each.  MORE: the row may be longer than the registers; the pieces beyond are read
-// twice, once into a running maximum and sum, and once for the gradient.
+// 16-byte pieces (fewer than G values) goes to the first lanes, one value each.  MORE: the row may be longer than the registers; the pieces beyond are read in
+// batches, and for the gradient once more.  Workgroups stay for row after row; the rows of a pass over the grid are turned by `turn`, so that sequences padded at
+// the same places do not leave some workgroups all the padding.  With 1024 lanes only one workgroup fits a CU, and it asks for its next row's pieces as it
+// writes the last's gradient: otherwise memory would wait for the sums and the sums for memory.
 template <typename T, int G, int NV, Mode MODE, bool MORE>
 __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
     using P = Pack<T>;
-    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64;
+    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = 2;
+    constexpr bool AHEAD = G == 1024;
     __shared__ float red[3][W], sums[RPB][STATS];
     const int lane = G <= 64 ? threadIdx.x % G : threadIdx.x, sub = G <= 64 ? threadIdx.x / G : 0;
-    const int A = g.p.n_actions, whole = A / N, rest = A - whole * N;
-    float st[STATS] = {};
-    for (int row = blockIdx.x * RPB + sub; row < g.p.rows; row += gridDim.x * RPB) {
-        const T* x = (const T*)g.p.logits + (int64_t)row * g.p.ld;
+    const int A = g.p.n_actions, whole = A / N, rest = A - whole * N, groups = (g.p.rows + RPB - 1) / RPB;
+    const float k = g.k;
+    u32x4 v[NV];
+    if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] = 0.f;   // (kept by the row's first lane)
+    auto row_at = [&](int pass) { return (pass * (int)gridDim.x + (int)((blockIdx.x + (unsigned)pass * g.turn) % gridDim.x)) * RPB + sub; };
+    auto logits = [&](int row) { return (const T*)g.p.logits + (int64_t)row * g.p.ld; };
+    int row = row_at(0), a = -1; float w = 0.f;
+    auto look = [&](int row, int& a, float& w) {          // a row beyond the last is left out
+        a = -1; w = 0.f;
+        if (row < g.p.rows) { a = g.p.actions[row]; w = MODE == LOSS && g.loss.weights ? g.loss.weights[row] : 1.f; }
+    };
+    auto counts = [&](int a, float w) { return a >= 0 && a < A && w != 0.f; };
+    // piece i of the lane: a base that all lanes share (scalar registers) and one offset for all i
+    const uint32_t at = (uint32_t)lane * 16u;
+    auto fetch = [&](const T* x, int i) { if (lane < whole - i * G) v[i] = *(const u32x4_any*)((const char*)x + i * G * 16 + at); };
+    look(row, a, w);
+    for (int pass = 0; pass * (int)gridDim.x < groups; pass++) {
+        const T* x = logits(row);
+        const int next = row_at(pass + 1);
+        int next_a; float next_w;
+        const bool last = (pass + 1) * (int)gridDim.x >= groups;
+        if (last) { next_a = -1; next_w = 0.f; } else look(next, next_a, next_w);
         const uint8_t* mask = g.p.mask ? g.p.mask + (int64_t)row * g.p.ld_mask : nullptr;
         T* dx = (T*)g.dlogits + (int64_t)row * g.ldd;
-        const int a = g.p.actions[row];
-        const float w = MODE == LOSS && g.loss.weights ? g.loss.weights[row] : 1.f;
-        bool on = a >= 0 && a < A && w != 0.f;
-        auto one = [&](int i) -> float { return mask && !mask[i] ? -INFINITY : (float)x[i]; };
-        auto piece = [&](int c) -> u32x4 { u32x4 v = *(const u32x4_any*)(x + c * N); if (mask) v = P::forbid(v, P::bytes(mask + c * N)); return v; };
-        float logp = 0.f, H = 0.f, c = 0.f, h = 0.f, mc = 0.f, L = 0.f, lpa = 0.f;
-        u32x4 v[NV]; float xt = -INFINITY;
+        bool on = counts(a, w);
+        const bool here = row < g.p.rows;
+        auto one = [&](int i) -> float { return mask && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; };
+        auto piece = [&](int c) -> u32x4 { u32x4 q = *(const u32x4_any*)(x + c * N); if (mask) q = P::forbid(q, P::bytes(mask + c * N)); return q; };
+        float logp = 0.f, H = 0.f, c = 0.f, h = 0.f, m = 0.f, L = 0.f, lpa = 0.f;
+        float xt = P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
+        bool careful = false;
         if (on) {
+            if (!AHEAD || pass == 0) {
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                v[i] = u32x4{P::NEG_INF, P::NEG_INF, P::NEG_INF, P::NEG_INF};
-                if (lane + i * G < whole) v[i] = *(const u32x4_any*)(x + (lane + i * G) * N);
-            }
-            if (mask) {
-                typename P::Bytes b[NV];
-#pragma unroll
-                for (int i = 0; i < NV; i++) { b[i] = 0; if (lane + i * G < whole) b[i] = P::bytes(mask + (lane + i * G) * N); }
-#pragma unroll
-                for (int i = 0; i < NV; i++) { v[i] = P::forbid(v[i], b[i]); __builtin_amdgcn_sched_barrier(0); }
+                for (int i = 0; i < NV; i++) { v[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; fetch(x, i); }
             }
             if (lane < rest) xt = one(whole * N + lane);
             const float xa = one(a);
-            float m = xt, S = 0.f, Wt = 0.f, more_mc = 0.f;
-            if (MORE) {
-                m = -INFINITY;
-                for (int k = lane + NV * G; k < whole; k += G) {
-                    const u32x4 q = piece(k);
-                    float top = P::get(q, 0);
+            if (mask) {
+                typename P::Bytes b[NV];
 #pragma unroll
-                    for (int j = 1; j < N; j++) top = fmaxf(top, P::get(q, j));
-                    if (top > m) {                        // (what is summed so far moves to the new maximum: S 2^(old - new), and W with each t)
-                        const float to = fabsf(top * g.k) < 3e38f ? top * g.k : 0.f, by = more_mc - to, f = S > 0.f ? __builtin_amdgcn_exp2f(by) : 0.f;
-                        Wt = f * (Wt + S * by); S *= f; m = top; more_mc = to;
-                    }
+                for (int i = 0; i < NV; i++) { b[i] = ~(typename P::Bytes)0; if (lane < whole - i * G) b[i] = P::bytes(mask + i * G * N + at / (16 / N)); }
 #pragma unroll
-                    for (int j = 0; j < N; j++) {
-                        const float t = fmaf(P::get(q, j), g.k, -more_mc), e = __builtin_amdgcn_exp2f(t);
-                        S += e; Wt = fmaf(e, fmaxf(t, -1e30f), Wt);
-                    }
-                }
-                m = fmaxf(m, xt);
+                for (int i = 0; i < NV; i++) { v[i] = P::forbid(v[i], b[i]); piece_done(); }
             }
+            RowSum r;
+            auto sum = [&](auto careful) {
+                constexpr bool CAREFUL = decltype(careful)::value;
+                r.clear();
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
+                for (int i = 0; i < NV; i++) r.template piece<CAREFUL, P>(v[i], k);
+                if (MORE)
+                    for (int p = lane + NV * G; p < whole; p += BATCH * G) {
+                        u32x4 q[BATCH];
 #pragma unroll
-                for (int j = 0; j < N; j += 2) m = max3(m, P::get(v[i], j), P::get(v[i], j + 1));
-                piece_done(v[i], m);
-            }
-            if (G <= 64) m = lanes<G, Max>(m);
-            else { put_wave<G, Max>(m, red[0]); __syncthreads(); m = get_waves<G, Max>(red[0]); }
-            // a row without an allowed action (or one of NaN alone: the maximum passes over NaN) is summed against 0: it gives 0 or NaN
-            const bool live = m > Lowest<T>::value && fabsf(m * g.k) < 3e38f;
-            mc = live ? m * g.k : 0.f;
-            if (MORE && S != 0.f) { const float by = more_mc - mc, f = __builtin_amdgcn_exp2f(by); Wt = f * (Wt + S * by); S *= f; }
-            float S4[4] = {S, 0.f, 0.f, 0.f}, W4[4] = {Wt, 0.f, 0.f, 0.f};
-            auto add = [&](float xv, int j) {
-                const float t = fmaf(xv, g.k, -mc), e = __builtin_amdgcn_exp2f(t);
-                S4[j & 3] += e; W4[j & 3] = fmaf(e, fmaxf(t, -1e30f), W4[j & 3]);        // (e = 0 where t is -inf)
+                        for (int i = 0; i < BATCH; i++) { q[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; if (p + i * G < whole) q[i] = piece(p + i * G); }
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++) r.template piece<CAREFUL, P>(q[i], k);
+                    }
+                r.reach(xt, k);
+                r.template add<CAREFUL>(xt, k, 1);
             };
-#pragma unroll
-            for (int i = 0; i < NV; i++) {
-#pragma unroll
-                for (int j = 0; j < N; j++) add(P::get(v[i], j), j);
-                piece_done(v[i], S4, W4);
-            }
-            add(xt, 3);
-            S = (S4[0] + S4[1]) + (S4[2] + S4[3]); Wt = (W4[0] + W4[1]) + (W4[2] + W4[3]);
+            sum(std::false_type{});
+            float Wt = r.w[0] + r.w[1];
+            careful = !(fabsf(Wt) < INFINITY);
+            if (careful) { sum(std::true_type{}); Wt = r.w[0] + r.w[1]; }
+            float S = r.s[0] + r.s[1];
+            // the lanes' sums against the row's m
+            if (G <= 64) m = lanes<G, Max>(r.m);
+            else { put_wave<G, Max>(r.m, red[0]); __syncthreads(); m = get_waves<G, Max>(red[0]); }
+            const float by = r.m - m, f = __builtin_amdgcn_exp2f(by);
+            Wt = f * fmaf(S, by, Wt); S *= f;
             if (G <= 64) { S = lanes<G, Sum>(S); Wt = lanes<G, Sum>(Wt); }
             else {
                 put_wave<G, Sum>(S, red[1]); put_wave<G, Sum>(Wt, red[2]);
                 __syncthreads();
                 S = get_waves<G, Sum>(red[1]); Wt = get_waves<G, Sum>(red[2]);
             }
-            if (!live) { on = S != 0.f; S = NAN; }
+            if (!(m > g.no_m)) on = S != S;               // nothing is allowed, but a NaN shows
             if (on) {
                 L = log2f(S);
                 H = LN2 * (L - Wt / S);
-                lpa = LN2 * (fmaf(xa, g.k, -mc) - L);
-                H = H < 0.f ? 0.f : H;                                   // (the rounding of mc can leave either an ulp of t off; a NaN stays)
+                lpa = LN2 * (fmaf(xa, k, -m) - L);
+                H = H < 0.f ? 0.f : H;                                   // (the rounding of m can leave either an ulp of t off; a NaN stays)
                 lpa = lpa > 0.f ? 0.f : (lpa < -1e30f ? -1e30f : lpa);   // (-inf: below every floor, and 0 times it is wanted below)
                 const bool floored = lpa < g.log_floor;
                 logp = floored ? g.log_floor : lpa;
                 if (MODE == BACKWARD) { c = floored ? 0.f : g.d_logp[row]; h = g.d_entropy ? g.d_entropy[row] : 0.f; }
-                if (MODE == LOSS) loss_row(g, row, w, logp, H, floored, c, h, st);
+                if (MODE == LOSS) {
+                    float st[STATS];
+                    loss_row(g, row, w, logp, H, floored, c, h, st);
+                    if (lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] += st[j];
+                }
             }
         }
-        if (lane == 0) {
+        const bool ahead = AHEAD && counts(next_a, next_w);
+        const T* next_x = logits(ahead ? next : 0);
+        if (here && lane == 0) {
             if (g.logp) g.logp[row] = logp;
             if (g.entropy) g.entropy[row] = H;
         }
-        if (MODE == LOGP || !g.dlogits) continue;
-        if (!on) {
-            for (int k = lane; k < whole; k += G) *(u32x4_any*)(dx + k * N) = u32x4{0, 0, 0, 0};
-            if (lane < rest) dx[whole * N + lane] = (T)0.f;
-            continue;
+        if (MODE == LOGP || !g.dlogits || !here || !on) {
+            if (ahead) {
+#pragma unroll
+                for (int i = 0; i < NV; i++) { v[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; fetch(next_x, i); }
+            }
+            if (MODE != LOGP && g.dlogits && here) {
+                for (int p = lane; p < whole; p += G) *(u32x4_any*)(dx + p * N) = u32x4{0, 0, 0, 0};
+                if (lane < rest) dx[whole * N + lane] = (T)0.f;
+            }
+        } else {
+            // e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i); the action's own c / T comes in a store of its own behind it
+            const float inv = g.inv_t * __builtin_amdgcn_exp2f(-L), p1 = -h * LN2 * inv, p0 = -(c + h * (H - LN2 * L)) * inv;
+            auto grad = [&](float xv) -> float { const float t = fmaf(xv, k, -m); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); };
+            auto grad_careful = [&](float xv) -> float { const float t = fmaxf(fmaf(xv, k, -m), -1e30f); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); };
+            auto store = [&](char* to, u32x4 q) {
+                float d[N];
+                if (careful) {
+#pragma unroll
+                    for (int j = 0; j < N; j++) d[j] = grad_careful(P::get(q, j));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j++) d[j] = grad(P::get(q, j));
+                }
+                *(u32x4_any*)to = P::put(d);
+            };
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                if (lane < whole - i * G) store((char*)dx + i * G * 16 + at, v[i]);
+                if (ahead) fetch(next_x, i);
+                piece_done();
+            }
+            if (MORE)
+                for (int p = lane + NV * G; p < whole; p += BATCH * G) {
+                    u32x4 q[BATCH];
+#pragma unroll
+                    for (int i = 0; i < BATCH; i++) if (p + i * G < whole) q[i] = piece(p + i * G);
+#pragma unroll
+                    for (int i = 0; i < BATCH; i++) { if (p + i * G < whole) store((char*)(dx + (p + i * G) * N), q[i]); piece_done(); }
+                }
+            if (lane < rest) dx[whole * N + lane] = (T)grad_careful(xt);
+            const int pa = a / N;
+            if (lane == (pa < whole ? pa % G : a - whole * N))
+                dx[a] = (T)((-c * expm1f(lpa) - h * expf(lpa) * (lpa + H)) * g.inv_t);       // c (1 - s) - h s (log s + H): its lane wrote the 16 bytes around it
         }
-        // e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i); the action's own c / T comes in a store of its own behind it
-        const float inv = g.inv_t * __builtin_amdgcn_exp2f(-L), p1 = -h * LN2 * inv, p0 = -(c + h * (H - LN2 * L)) * inv;
-        auto grad = [&](float xv) -> float { const float t = fmaxf(fmaf(xv, g.k, -mc), -1e30f); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); };
-        auto store = [&](int k, u32x4 q) {
-            float d[N];
-#pragma unroll
-            for (int j = 0; j < N; j++) d[j] = grad(P::get(q, j));
-            *(u32x4_any*)(dx + k * N) = P::put(d);
-        };
-#pragma unroll
-        for (int i = 0; i < NV; i++) { if (lane + i * G < whole) store(lane + i * G, v[i]); __builtin_amdgcn_sched_barrier(0); }
-        if (MORE) for (int k = lane + NV * G; k < whole; k += G) store(k, piece(k));
-        if (lane < rest) dx[whole * N + lane] = (T)grad(xt);
-        const int ka = a / N;
-        if (lane == (ka < whole ? ka % G : a - whole * N))
-            dx[a] = (T)((-c * expm1f(lpa) - h * expf(lpa) * (lpa + H)) * g.inv_t);       // c (1 - s) - h s (log s + H): its lane wrote the 16 bytes around it
+        row = next; a = next_a; w = next_w;
     }
     if (MODE != LOSS) return;
-    if (lane == 0) for (int k = 0; k < STATS; k++) sums[sub][k] = st[k];
     __syncthreads();
     if (threadIdx.x < STATS) {
         float s = sums[0][threadIdx.x];
-        for (int k = 1; k < RPB; k++) s += sums[k][threadIdx.x];
+        for (int j = 1; j < RPB; j++) s += sums[j][threadIdx.x];
         g.row_stats[(int64_t)blockIdx.x * STATS + threadIdx.x] = s;
     }
 }
@@ -426,13 +487,17 @@ RowArgs row_args(const RlgpuPolicyRows* p) {
     return g;
 }
 // Lanes and 16-byte pieces a row: the smallest set of registers that holds it.  Workgroups: as many as the device keeps at once, each taking rows in turn.
-template <typename T, Mode MODE> int launch_rows_of(const RowArgs& g, hipStream_t s, int& blocks) {
+template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, int& blocks) {
     const int whole = g.p.n_actions / Pack<T>::N;
+    const uint32_t fill = Pack<T>::FILL; float low;
+    if (sizeof(T) == 2 && fill == 0xfbfffbffu) low = -65504.f; else { const uint32_t f = fill & 0xffff0000u; std::memcpy(&low, &f, 4); }
+    g.no_m = std::max(low * g.k, NO_M);
 #define ROWS(G, NV, MORE)                                                                                                        \
     do {                                                                                                                         \
         if (MORE || whole <= (G) * (NV)) {                                                                                       \
             const int rpb = (G) <= 64 ? 256 / (G) : 1;                                                                           \
-            blocks = std::min(ROW_BLOCKS, (g.p.rows + rpb - 1) / rpb);                                                           \
+            blocks = std::min((G) == 1024 ? BLOCKS_OF_1024 : ROW_BLOCKS, (g.p.rows + rpb - 1) / rpb);                            \
+            g.turn = blocks * 5u / 13u;                                                                                          \
             hipLaunchKernelGGL((k_rows<T, G, NV, MODE, MORE>), dim3(blocks), dim3((G) <= 64 ? 256 : (G)), 0, s, g);              \
             OCHK(hipGetLastError());                                                                                             \
             return RLGPU_OK;                                                                                                     \

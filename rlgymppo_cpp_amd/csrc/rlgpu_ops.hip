@@ -21,7 +21,7 @@
 namespace {
 
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
-constexpr int STATS = RLGPU_POLICY_STATS, ROW_BLOCKS = 2048, BLOCKS_OF_1024 = 256;
+constexpr int STATS = RLGPU_POLICY_STATS, ROW_BLOCKS = 2048;
 
 // what a launch over rows takes; mode decides which of the outputs are there
 struct RowArgs {
@@ -184,7 +184,7 @@ template <int G, typename OP> __device__ __forceinline__ float get_waves(const f
 template <typename T, int G, int NV, Mode MODE, bool MORE>
 __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
     using P = Pack<T>;
-    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = 2;
+    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = MODE == LOGP ? 4 : 2;
     constexpr bool AHEAD = G == 1024;
     __shared__ float red[3][W], sums[RPB][STATS];
     const int lane = G <= 64 ? threadIdx.x % G : threadIdx.x, sub = G <= 64 ? threadIdx.x / G : 0;
@@ -344,17 +344,27 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
     }
 }
 
-// the workgroups' statistics in a fixed order: 64 slices of them, then the slices, in 64 bits
-__global__ void __launch_bounds__(512) k_row_stats(const float* part, int n, float* stats) {
-    __shared__ double red[512];
-    const int k = threadIdx.x & 7;
-    double s = 0;
-    for (int i = threadIdx.x >> 3; i < n; i += 64) s += (double)part[i * STATS + k];
-    red[threadIdx.x] = s;
+// The workgroups' statistics in a fixed order, in 64 bits: thread t adds the float4 t, t + 1024, ... (its four statistics of every 512th workgroup), the lanes of
+// like statistics are joined by xor, and the wavefronts in order.
+__global__ void __launch_bounds__(1024) k_row_stats(const float4* part, int n, float* stats) {
+    __shared__ double red[16][STATS];
+    const int tid = threadIdx.x;
+    double s[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 2 * ROW_BLOCKS / 1024; i++) {
+        const int at = tid + i * 1024;
+        const float4 v = at < 2 * n ? part[at] : float4{0.f, 0.f, 0.f, 0.f};
+        s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+    }
+#pragma unroll
+    for (int o = 32; o > 1; o >>= 1) for (int j = 0; j < 4; j++) s[j] += __shfl_xor(s[j], o, 64);
+    if ((tid & 63) < 2) for (int j = 0; j < 4; j++) red[tid >> 6][(tid & 1) * 4 + j] = s[j];
     __syncthreads();
-    if (threadIdx.x < STATS) {
-        for (int j = 1; j < 64; j++) s += red[j * STATS + k];
-        stats[k] = (float)s;
+    if (tid < STATS) {
+        double sum = red[0][tid];
+#pragma unroll
+        for (int j = 1; j < 16; j++) sum += red[j][tid];
+        stats[tid] = (float)sum;
     }
 }
 
@@ -486,27 +496,43 @@ RowArgs row_args(const RlgpuPolicyRows* p) {
     g.inv_t = 1.f / p->temperature; g.k = (float)(1.4426950408889634 / (double)p->temperature); g.log_floor = (float)std::log((double)p->min_prob);
     return g;
 }
-// Lanes and 16-byte pieces a row: the smallest set of registers that holds it.  Workgroups: as many as the device keeps at once, each taking rows in turn.
+// workgroups of a kernel that the device keeps at once (a second, partly filled round would leave most of it idle)
+template <typename K> int resident(K kernel, int threads) {
+    int device = 0, cus = 256, per_cu = 1;
+    (void)hipGetDevice(&device);
+    (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess) { (void)hipGetLastError(); per_cu = 1; }
+    return std::max(1, std::min(ROW_BLOCKS, cus * per_cu));
+}
+template <typename T, int G, int NV, Mode MODE, bool MORE> int launch_rows_as(RowArgs& g, hipStream_t s, int& blocks) {
+    constexpr int threads = G <= 64 ? 256 : G, rpb = threads / G;
+    static const int most = resident(&k_rows<T, G, NV, MODE, MORE>, threads);
+    blocks = std::min(most, (g.p.rows + rpb - 1) / rpb);
+    g.turn = blocks * 5u / 13u;
+    hipLaunchKernelGGL((k_rows<T, G, NV, MODE, MORE>), dim3(blocks), dim3(threads), 0, s, g);
+    OCHK(hipGetLastError());
+    return RLGPU_OK;
+}
+// Lanes and 16-byte pieces a row: the smallest set of registers that holds it.  Sums alone need no more of a row than what is in flight: 256 lanes take any.
 template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, int& blocks) {
     const int whole = g.p.n_actions / Pack<T>::N;
     const uint32_t fill = Pack<T>::FILL; float low;
     if (sizeof(T) == 2 && fill == 0xfbfffbffu) low = -65504.f; else { const uint32_t f = fill & 0xffff0000u; std::memcpy(&low, &f, 4); }
     g.no_m = std::max(low * g.k, NO_M);
-#define ROWS(G, NV, MORE)                                                                                                        \
-    do {                                                                                                                         \
-        if (MORE || whole <= (G) * (NV)) {                                                                                       \
-            const int rpb = (G) <= 64 ? 256 / (G) : 1;                                                                           \
-            blocks = std::min((G) == 1024 ? BLOCKS_OF_1024 : ROW_BLOCKS, (g.p.rows + rpb - 1) / rpb);                            \
-            g.turn = blocks * 5u / 13u;                                                                                          \
-            hipLaunchKernelGGL((k_rows<T, G, NV, MODE, MORE>), dim3(blocks), dim3((G) <= 64 ? 256 : (G)), 0, s, g);              \
-            OCHK(hipGetLastError());                                                                                             \
-            return RLGPU_OK;                                                                                                     \
-        }                                                                                                                        \
-    } while (0)
-    ROWS(16, 1, false); ROWS(16, 2, false); ROWS(64, 1, false); ROWS(64, 2, false); ROWS(64, 4, false);
-    ROWS(256, 2, false); ROWS(256, 4, false); ROWS(256, 8, false); ROWS(1024, 4, false); ROWS(1024, 8, false); ROWS(1024, 16, true);
-#undef ROWS
-    return RLGPU_OK;
+    if (whole <= 16) return launch_rows_as<T, 16, 1, MODE, false>(g, s, blocks);
+    if (whole <= 16 * 2) return launch_rows_as<T, 16, 2, MODE, false>(g, s, blocks);
+    if (whole <= 64) return launch_rows_as<T, 64, 1, MODE, false>(g, s, blocks);
+    if (whole <= 64 * 2) return launch_rows_as<T, 64, 2, MODE, false>(g, s, blocks);
+    if (whole <= 64 * 4) return launch_rows_as<T, 64, 4, MODE, false>(g, s, blocks);
+    if (whole <= 256 * 2) return launch_rows_as<T, 256, 2, MODE, false>(g, s, blocks);
+    if constexpr (MODE == LOGP) return launch_rows_as<T, 256, 4, LOGP, true>(g, s, blocks);
+    else {
+        if (whole <= 256 * 4) return launch_rows_as<T, 256, 4, MODE, false>(g, s, blocks);
+        if (whole <= 256 * 8) return launch_rows_as<T, 256, 8, MODE, false>(g, s, blocks);
+        if (whole <= 1024 * 4) return launch_rows_as<T, 1024, 4, MODE, false>(g, s, blocks);
+        if (whole <= 1024 * 8) return launch_rows_as<T, 1024, 8, MODE, false>(g, s, blocks);
+        return launch_rows_as<T, 1024, 16, MODE, true>(g, s, blocks);
+    }
 }
 template <Mode MODE> int launch_rows(const RowArgs& g, hipStream_t s, int& blocks) {
     blocks = 0;
@@ -574,7 +600,7 @@ int rlgpu_policy_loss(int device, const RlgpuPolicyRows* p, const RlgpuPolicyLos
     g.loss = *l; g.logp = l->logp; g.dlogits = l->dlogits; g.ldd = l->ld_dlogits; g.row_stats = (float*)workspace;
     int blocks;
     if (int rc = launch_rows<LOSS>(g, (hipStream_t)stream, blocks)) return rc;
-    hipLaunchKernelGGL(k_row_stats, dim3(1), dim3(512), 0, (hipStream_t)stream, (const float*)workspace, blocks, l->stats);
+    hipLaunchKernelGGL(k_row_stats, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const float4*)workspace, blocks, l->stats);
     OCHK(hipGetLastError());
     return RLGPU_OK;
 }

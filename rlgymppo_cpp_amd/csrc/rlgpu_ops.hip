@@ -37,18 +37,19 @@ struct RowArgs {
 };
 enum Mode { LOGP, BACKWARD, LOSS };
 
+// e^x by the hardware's 2^x: off by an ulp and by the rounding of x log2(e), |x| 2^-24, which is what a difference of log-probabilities is off by already
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 // exp(x) - 1 - x: near 0 by its series (the terms left out are under 2^-26 of the first), since the subtraction would cancel there
 __device__ __forceinline__ float exp_minus_1_minus(float x) {
-    if (fabsf(x) < 0.25f)
-        return x * x * (0.5f + x * (1.f / 6 + x * (1.f / 24 + x * (1.f / 120 + x * (1.f / 720 + x * (1.f / 5040 + x * (1.f / 40320)))))));
-    return expf(x) - 1.f - x;
+    const float near = x * x * (0.5f + x * (1.f / 6 + x * (1.f / 24 + x * (1.f / 120 + x * (1.f / 720 + x * (1.f / 5040 + x * (1.f / 40320)))))));
+    return fabsf(x) < 0.25f ? near : exp_of(x) - 1.f - x;
 }
 
 // one row of the loss: d loss / d logp and d loss / d entropy, and the row's part of the statistics
 __device__ void loss_row(const RowArgs& g, int row, float w, float logp, float H, bool floored, float& c, float& h, float (&st)[STATS]) {
     const RlgpuPolicyLoss& l = g.loss;
     const float x = logp - l.old_logp[row], adv = l.adv[row];
-    const float r = expf(x);
+    const float r = exp_of(x);
     const float surr = r * adv, clipped = fminf(fmaxf(r, 1.f - l.clip_low), 1.f + l.clip_high) * adv;
     float value = -(clipped < surr ? clipped : surr);     // (a NaN in either stays: surr holds it)
     c = clipped < surr ? 0.f : -surr;
@@ -57,7 +58,7 @@ __device__ void loss_row(const RowArgs& g, int row, float w, float logp, float H
         const float d = l.ref_logp[row] - logp;
         ref = exp_minus_1_minus(d);
         value += l.kl_coef * ref;
-        c -= l.kl_coef * expm1f(d);
+        c -= l.kl_coef * (ref + d);                       // exp(d) - 1
     }
     value -= l.ent_coef * H;
     c = floored ? 0.f : c * w * l.scale;
@@ -158,20 +159,25 @@ struct RowSum {
     }
 };
 
-// ---- sums and maxima over the G lanes of a row; G = 16 stays in a DPP row, more than 64 goes through LDS (`red`: one float a wavefront) ----------------------
-template <int CTRL> __device__ __forceinline__ float dpp(float v) {
-    const int i = __builtin_bit_cast(int, v);
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
-}
-struct Sum { static __device__ __forceinline__ float of(float a, float b) { return a + b; } };
-struct Max { static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); } };
-template <int N, typename OP> __device__ __forceinline__ float lanes(float v) {       // over aligned groups of N lanes, every lane gets the result
+// ---- sums and maxima over the G lanes of a row; G <= 16 stays in a DPP row, more than 64 goes through LDS (`red`: one float a wavefront) ----------------------
+// (a bound-checked move of a lane that is always there: the compiler folds it into the operation)
+template <int CTRL> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
+struct Sum { static __device__ __forceinline__ int of(int a, int b) { return __builtin_bit_cast(int, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b)); } };
+struct Max { static __device__ __forceinline__ int of(int a, int b) { return max(a, b); } };        // of in_order()
+template <int N, typename OP> __device__ __forceinline__ int lanes_of(int v) {        // over aligned groups of N lanes, every lane gets the result
     v = OP::of(v, dpp<0xB1>(v));                          // quad_perm 1 0 3 2
     if (N > 2) v = OP::of(v, dpp<0x4E>(v));               // quad_perm 2 3 0 1
     if (N > 4) v = OP::of(v, dpp<0x141>(v));              // row_half_mirror
     if (N > 8) v = OP::of(v, dpp<0x140>(v));              // row_mirror
     if (N > 16) { v = OP::of(v, __shfl_xor(v, 16, 64)); v = OP::of(v, __shfl_xor(v, 32, 64)); }
     return v;
+}
+// floats as integers of the same order (their own inverse): maxima of integers need no quieting of NaN, which none of these is
+__device__ __forceinline__ int in_order(int i) { return i ^ ((i >> 31) & 0x7fffffff); }
+template <int N, typename OP> __device__ __forceinline__ float lanes(float f) {
+    const int v = __builtin_bit_cast(int, f);
+    if constexpr (std::is_same_v<OP, Max>) return __builtin_bit_cast(float, in_order(lanes_of<N, Max>(in_order(v))));
+    else return __builtin_bit_cast(float, lanes_of<N, Sum>(v));
 }
 template <int G, typename OP> __device__ __forceinline__ void put_wave(float v, float* red) { v = lanes<64, OP>(v); if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v; }
 template <int G, typename OP> __device__ __forceinline__ float get_waves(const float* red) { constexpr int W = G / 64; return lanes<W, OP>(red[threadIdx.x & (W - 1)]); }
@@ -190,6 +196,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
     const int lane = G <= 64 ? threadIdx.x % G : threadIdx.x, sub = G <= 64 ? threadIdx.x / G : 0;
     const int A = g.p.n_actions, whole = A / N, rest = A - whole * N, groups = (g.p.rows + RPB - 1) / RPB;
     const float k = g.k;
+    const bool masked = g.p.mask != nullptr;
     u32x4 v[NV];
     if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] = 0.f;   // (kept by the row's first lane)
     auto row_at = [&](int pass) { return (pass * (int)gridDim.x + (int)((blockIdx.x + (unsigned)pass * g.turn) % gridDim.x)) * RPB + sub; };
@@ -210,12 +217,12 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
         int next_a; float next_w;
         const bool last = (pass + 1) * (int)gridDim.x >= groups;
         if (last) { next_a = -1; next_w = 0.f; } else look(next, next_a, next_w);
-        const uint8_t* mask = g.p.mask ? g.p.mask + (int64_t)row * g.p.ld_mask : nullptr;
+        const uint8_t* mask = g.p.mask + (int64_t)row * g.p.ld_mask;
         T* dx = (T*)g.dlogits + (int64_t)row * g.ldd;
         bool on = counts(a, w);
         const bool here = row < g.p.rows;
-        auto one = [&](int i) -> float { return mask && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; };
-        auto piece = [&](int c) -> u32x4 { u32x4 q = *(const u32x4_any*)(x + c * N); if (mask) q = P::forbid(q, P::bytes(mask + c * N)); return q; };
+        auto one = [&](int i) -> float { return masked && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; };
+        auto piece = [&](int c) -> u32x4 { u32x4 q = *(const u32x4_any*)(x + c * N); if (masked) q = P::forbid(q, P::bytes(mask + c * N)); return q; };
         float logp = 0.f, H = 0.f, c = 0.f, h = 0.f, m = 0.f, L = 0.f, lpa = 0.f;
         float xt = P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
         bool careful = false;
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
             }
             if (lane < rest) xt = one(whole * N + lane);
             const float xa = one(a);
-            if (mask) {
+            if (masked) {
                 typename P::Bytes b[NV];
 #pragma unroll
                 for (int i = 0; i < NV; i++) { b[i] = ~(typename P::Bytes)0; if (lane < whole - i * G) b[i] = P::bytes(mask + i * G * N + at / (16 / N)); }
@@ -268,8 +275,8 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
             }
             if (!(m > g.no_m)) on = S != S;               // nothing is allowed, but a NaN shows
             if (on) {
-                L = log2f(S);
-                H = LN2 * (L - Wt / S);
+                L = __builtin_amdgcn_logf(S);            // (log2; S is about 1 at least)
+                H = LN2 * (L - Wt * __builtin_amdgcn_rcpf(S));
                 lpa = LN2 * (fmaf(xa, k, -m) - L);
                 H = H < 0.f ? 0.f : H;                                   // (the rounding of m can leave either an ulp of t off; a NaN stays)
                 lpa = lpa > 0.f ? 0.f : (lpa < -1e30f ? -1e30f : lpa);   // (-inf: below every floor, and 0 times it is wanted below)
@@ -331,7 +338,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
             if (lane < rest) dx[whole * N + lane] = (T)grad_careful(xt);
             const int pa = a / N;
             if (lane == (pa < whole ? pa % G : a - whole * N))
-                dx[a] = (T)((-c * expm1f(lpa) - h * expf(lpa) * (lpa + H)) * g.inv_t);       // c (1 - s) - h s (log s + H): its lane wrote the 16 bytes around it
+                dx[a] = (T)((c - exp_of(lpa) * (c + h * (lpa + H))) * g.inv_t);       // its lane wrote the 16 bytes around it
         }
         row = next; a = next_a; w = next_w;
     }
@@ -519,12 +526,14 @@ template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, in
     const uint32_t fill = Pack<T>::FILL; float low;
     if (sizeof(T) == 2 && fill == 0xfbfffbffu) low = -65504.f; else { const uint32_t f = fill & 0xffff0000u; std::memcpy(&low, &f, 4); }
     g.no_m = std::max(low * g.k, NO_M);
-    if (whole <= 16) return launch_rows_as<T, 16, 1, MODE, false>(g, s, blocks);
-    if (whole <= 16 * 2) return launch_rows_as<T, 16, 2, MODE, false>(g, s, blocks);
-    if (whole <= 64) return launch_rows_as<T, 64, 1, MODE, false>(g, s, blocks);
+    if (whole <= 8) return launch_rows_as<T, 8, 1, MODE, false>(g, s, blocks);
+    if (whole <= 8 * 2) return launch_rows_as<T, 8, 2, MODE, false>(g, s, blocks);
+    if (whole <= 8 * 3) return launch_rows_as<T, 8, 3, MODE, false>(g, s, blocks);
+    if (whole <= 8 * 4) return launch_rows_as<T, 8, 4, MODE, false>(g, s, blocks);
+    if (whole <= 16 * 4) return launch_rows_as<T, 16, 4, MODE, false>(g, s, blocks);
     if (whole <= 64 * 2) return launch_rows_as<T, 64, 2, MODE, false>(g, s, blocks);
     if (whole <= 64 * 4) return launch_rows_as<T, 64, 4, MODE, false>(g, s, blocks);
-    if (whole <= 256 * 2) return launch_rows_as<T, 256, 2, MODE, false>(g, s, blocks);
+    if (whole <= 64 * 8) return launch_rows_as<T, 64, 8, MODE, false>(g, s, blocks);
     if constexpr (MODE == LOGP) return launch_rows_as<T, 256, 4, LOGP, true>(g, s, blocks);
     else {
         if (whole <= 256 * 4) return launch_rows_as<T, 256, 4, MODE, false>(g, s, blocks);

@@ -386,18 +386,34 @@ struct ClipBatch {
 };
 static_assert(sizeof(ClipBatch) < 3900, "kernel arguments by value");
 
-template <typename F> __device__ __forceinline__ void for_pieces(const ClipBatch& b, F&& f) {
-    for (int piece = blockIdx.x; piece < b.first[b.n]; piece += gridDim.x) {
+// `from_end`: the pieces in the opposite order.  The second reading of the gradients begins with what the first read last and the caches still hold.
+template <typename F> __device__ __forceinline__ void for_pieces(const ClipBatch& b, bool from_end, F&& f) {
+    const int n = b.first[b.n];
+    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+        const int piece = from_end ? n - 1 - i : i;
         int lo = 0, hi = b.n;                                          // the last tensor whose first piece is <= piece (empty tensors share their successor's)
         while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (b.first[mid] <= piece) lo = mid; else hi = mid; }
         const int64_t at = (int64_t)(piece - b.first[lo]) * PIECE;
         f(lo, at, (int)min((int64_t)PIECE, b.count[lo] - at));
     }
 }
+constexpr int IN_FLIGHT = 4;              // 16-byte loads of a lane
 template <typename T> __device__ __forceinline__ double square_sum(const T* g, int n) {
-    double s = 0;
-    for (int i = threadIdx.x; i < n; i += 256) { const double v = (double)(float)g[i]; s += v * v; }
-    return s;
+    using P = Pack<T>;
+    const int whole = n / P::N;
+    double s[2] = {0, 0};
+    for (int i = threadIdx.x; i < whole; i += IN_FLIGHT * 256) {
+        u32x4 v[IN_FLIGHT];
+#pragma unroll
+        for (int j = 0; j < IN_FLIGHT; j++) { v[j] = u32x4{0, 0, 0, 0}; if (i + j * 256 < whole) v[j] = *(const u32x4_any*)(g + (i + j * 256) * P::N); }
+#pragma unroll
+        for (int j = 0; j < IN_FLIGHT; j++)
+#pragma unroll
+            for (int e = 0; e < P::N; e++) { const double x = P::get(v[j], e); s[e & 1] = fma(x, x, s[e & 1]); }
+    }
+    const int i = whole * P::N + threadIdx.x;
+    if (i < n) { const double x = (float)g[i]; s[0] = fma(x, x, s[0]); }
+    return s[0] + s[1];
 }
 __device__ __forceinline__ double block_sum(double s, double* red) {
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -409,7 +425,7 @@ __device__ __forceinline__ double block_sum(double s, double* red) {
 __global__ void __launch_bounds__(256) k_grad_squares(ClipBatch b, double* part) {
     __shared__ double red[4];
     double s = 0;
-    for_pieces(b, [&](int t, int64_t at, int n) {
+    for_pieces(b, false, [&](int t, int64_t at, int n) {
         if (b.dtype[t] == RLGPU_F32) s += square_sum((const float*)b.g[t] + at, n);
         else if (b.dtype[t] == RLGPU_BF16) s += square_sum((const __bf16*)b.g[t] + at, n);
         else s += square_sum((const _Float16*)b.g[t] + at, n);
@@ -418,7 +434,22 @@ __global__ void __launch_bounds__(256) k_grad_squares(ClipBatch b, double* part)
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 template <typename T> __device__ __forceinline__ void scale_piece(T* g, int n, float f) {
-    for (int i = threadIdx.x; i < n; i += 256) g[i] = (T)((float)g[i] * f);
+    using P = Pack<T>;
+    const int whole = n / P::N;
+    for (int i = threadIdx.x; i < whole; i += IN_FLIGHT * 256) {
+        u32x4 v[IN_FLIGHT];
+#pragma unroll
+        for (int j = 0; j < IN_FLIGHT; j++) if (i + j * 256 < whole) v[j] = *(const u32x4_any*)(g + (i + j * 256) * P::N);
+#pragma unroll
+        for (int j = 0; j < IN_FLIGHT; j++) {
+            float d[P::N];
+#pragma unroll
+            for (int e = 0; e < P::N; e++) d[e] = P::get(v[j], e) * f;
+            if (i + j * 256 < whole) *(u32x4_any*)(g + (i + j * 256) * P::N) = P::put(d);
+        }
+    }
+    const int i = whole * P::N + threadIdx.x;
+    if (i < n) g[i] = (T)((float)g[i] * f);
 }
 // every workgroup adds the partial sums up itself, all in the same order: no launch in between
 __global__ void __launch_bounds__(256) k_grad_scale(ClipBatch b, const double* part, int n_part, float max_norm, float grad_scale, float* norm_out) {
@@ -430,7 +461,7 @@ __global__ void __launch_bounds__(256) k_grad_scale(ClipBatch b, const double* p
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const float f = (float)((double)grad_scale * fmin(1.0, (double)max_norm / (norm + 1e-6)));
     if (!(norm < INFINITY) || f == 1.f) return;
-    for_pieces(b, [&](int t, int64_t at, int n) {
+    for_pieces(b, true, [&](int t, int64_t at, int n) {
         if (b.dtype[t] == RLGPU_F32) scale_piece((float*)b.g[t] + at, n, f);
         else if (b.dtype[t] == RLGPU_BF16) scale_piece((__bf16*)b.g[t] + at, n, f);
         else scale_piece((_Float16*)b.g[t] + at, n, f);
@@ -671,11 +702,10 @@ int rlgpu_clip_grad_norm(int device, int32_t n, void* const* grads, const int64_
         OCHK(hipGetLastError());
         n_part += blocks;
     }
-    for (int k = 0; k < n_batches; k++) {
-        int blocks = batch(k, b);
-        if (!writes) { if (k) break; b.n = 0; b.first[0] = 0; blocks = 1; }   // the norm alone
-        if (k && blocks == 0) continue;
-        hipLaunchKernelGGL(k_grad_scale, dim3(std::max(1, blocks)), dim3(256), 0, s, b, (const double*)part, n_part, max_norm, grad_scale, k == 0 ? norm : (float*)nullptr);
+    for (int k = n_batches - 1; k >= 0; k--) {
+        int blocks = writes ? batch(k, b) : 0;
+        if (blocks == 0) { if (k) continue; b.n = 0; b.first[0] = 0; blocks = 1; }   // the last launch writes the norm, whatever there is to scale
+        hipLaunchKernelGGL(k_grad_scale, dim3(blocks), dim3(256), 0, s, b, (const double*)part, n_part, max_norm, grad_scale, k == 0 ? norm : (float*)nullptr);
         OCHK(hipGetLastError());
     }
     return RLGPU_OK;

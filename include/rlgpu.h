@@ -386,7 +386,7 @@ const char* rlgpu_lt_last_error(void);
  * streams as long as each has a workspace of its own.  The text of an error: rlgpu_ops_last_error() (of the calling thread). */
 enum { RLGPU_F32 = 0, RLGPU_BF16 = 1, RLGPU_F16 = 2 };
 typedef struct RlgpuPolicyRows {
-    const void* logits; int64_t ld;           /* [rows][n_actions], row stride `ld` in elements (>= n_actions), any alignment of a row */
+    const void* logits; int64_t ld;           /* [rows][n_actions], row stride `ld` in elements (n_actions .. 2^31), any alignment of a row */
     const uint8_t* mask; int64_t ld_mask;     /* optional [rows][n_actions]: 0 = the action is not allowed, its logit is not looked at (it may be NaN); ld_mask 0: one row for all */
     const int32_t* actions;                   /* [rows]; an index outside 0 .. n_actions - 1 leaves the row out */
     int32_t dtype, rows, n_actions;           /* RLGPU_F32 / BF16 / F16, rows >= 0, 1 <= n_actions <= 2^28 */
@@ -395,9 +395,10 @@ typedef struct RlgpuPolicyRows {
 /* Per row, over the allowed actions, with s = softmax(logits / temperature):
  *   logp = log max(s[action], min_prob)   (an action that is not allowed has s = 0),   entropy = -sum s log s   (0 log 0 = 0).
  * A row is LEFT OUT when its action is out of range or when nothing is allowed in it (mask all 0, or every allowed logit -inf or the type's lowest finite
- * value): logp = entropy = 0 and its gradient is zero.  NaN and +inf among the allowed logits give NaN; finite logits are taken up to |logit| / temperature < 2e38.
- * entropy may be NULL.  Workspace: rlgpu_policy_workspace bytes, 16-byte aligned, free again when the call's work on the stream is done. */
-int64_t rlgpu_policy_workspace(int32_t dtype, int32_t rows, int32_t n_actions);   /* bytes, for any of the three calls below; < 0: bad argument */
+ * value): logp = entropy = 0 and its gradient is zero.  NaN and +inf among the allowed logits give NaN.  Finite logits are taken within +-9e36 and
+ * |logit| / temperature < 2e38; what is below counts as -inf, what is above as +inf.
+ * entropy may be NULL.  Workspace: rlgpu_policy_workspace bytes (0: it may be NULL), 16-byte aligned, free again when the call's work on the stream is done. */
+int64_t rlgpu_policy_workspace(int32_t dtype, int32_t rows, int32_t n_actions, int32_t loss /* 1: for rlgpu_policy_loss, 0: for the other two */);   /* bytes; < 0: bad argument */
 int rlgpu_action_logp(int device, const RlgpuPolicyRows* p, float* logp, float* entropy, void* workspace, int64_t workspace_bytes, void* hip_stream);
 /* dlogits[rows][n_actions] (p->dtype, row stride ld_dlogits) = d(sum d_logp logp + d_entropy entropy) / d logits; d_entropy may be NULL (zero).  The floor
  * passes no gradient, actions that are not allowed get 0.  dlogits may be p->logits itself (same stride), else the two may not overlap. */

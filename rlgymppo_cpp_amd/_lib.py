@@ -189,7 +189,7 @@ SIGNATURES = {
     "rlgpu_lt_write_adam": (_i, [C.c_char_p, _vp, C.c_int, C.c_float, _vp, _vp, C.c_int64]),
     "rlgpu_lt_read_adam": (_i, [C.c_char_p, _vp, C.c_int, _vp, _vp, C.POINTER(C.c_int64)]),
     "rlgpu_lt_last_error": (C.c_char_p, []),
-    "rlgpu_policy_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
+    "rlgpu_policy_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "rlgpu_action_logp": (_i, [_i, C.POINTER(PolicyRows), _vp, _vp, _vp, C.c_int64, _vp]),
     "rlgpu_action_logp_backward": (_i, [_i, C.POINTER(PolicyRows), _vp, _vp, _vp, C.c_int64, _vp, C.c_int64, _vp]),
     "rlgpu_policy_loss": (_i, [_i, C.POINTER(PolicyRows), C.POINTER(PolicyLossC), _vp, C.c_int64, _vp]),

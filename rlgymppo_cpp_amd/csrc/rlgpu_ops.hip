@@ -33,7 +33,7 @@ struct RowArgs {
     const float *d_logp, *d_entropy;      // backward
     RlgpuPolicyLoss loss;                 // loss
     void* dlogits; int64_t ldd;           // optional
-    float* row_stats;                     // [workgroups][STATS]: each workgroup's sums over its rows
+    float* row_stats;                     // the workspace; the loss has [workgroups][STATS] in front: each workgroup's sums over its rows
 };
 enum Mode { LOGP, BACKWARD, LOSS };
 
@@ -182,6 +182,46 @@ template <int N, typename OP> __device__ __forceinline__ float lanes(float f) {
 template <int G, typename OP> __device__ __forceinline__ void put_wave(float v, float* red) { v = lanes<64, OP>(v); if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v; }
 template <int G, typename OP> __device__ __forceinline__ float get_waves(const float* red) { constexpr int W = G / 64; return lanes<W, OP>(red[threadIdx.x & (W - 1)]); }
 
+// What follows from a row's m, S and W and its action's logit: whether it counts, its outputs, and what its gradient needs.
+struct RowNumbers { float logp, H, lpa, L, c, h; bool on; };
+template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const RowArgs& g, int row, float w, float m, float S, float W, float xa, float (&st)[STATS]) {
+    RowNumbers n{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, true};
+    if (!(m > g.no_m)) n.on = S != S;                     // nothing is allowed, but a NaN shows
+    if (!n.on) return n;
+    n.L = __builtin_amdgcn_logf(S);                       // (log2; S is about 1 at least)
+    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (fmaf(xa, g.k, -m) - n.L);
+    n.H = H < 0.f ? 0.f : H;                              // (the rounding of m can leave either an ulp of t off; a NaN stays)
+    n.lpa = lpa > 0.f ? 0.f : (lpa < -1e30f ? -1e30f : lpa);             // (-inf: below every floor, and 0 times it is wanted)
+    const bool floored = n.lpa < g.log_floor;
+    n.logp = floored ? g.log_floor : n.lpa;
+    if (MODE == BACKWARD) { n.c = floored ? 0.f : g.d_logp[row]; n.h = g.d_entropy ? g.d_entropy[row] : 0.f; }
+    if (MODE == LOSS) loss_row(g, row, w, n.logp, n.H, floored, n.c, n.h, st);
+    return n;
+}
+// The gradient of a piece: e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i).  The action's own c / T comes in a store of its own, of the lane that
+// wrote the 16 bytes around it.
+struct RowGradient {
+    float k, m, p0, p1; bool careful;
+    __device__ __forceinline__ RowGradient(const RowArgs& g, const RowNumbers& n, float m, bool careful) : k(g.k), m(m), careful(careful) {
+        const float inv = g.inv_t * __builtin_amdgcn_exp2f(-n.L);
+        p1 = -n.h * LN2 * inv; p0 = -(n.c + n.h * (n.H - LN2 * n.L)) * inv;
+    }
+    __device__ __forceinline__ float quick(float x) const { const float t = fmaf(x, k, -m); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
+    __device__ __forceinline__ float of(float x) const { const float t = fmaxf(fmaf(x, k, -m), -1e30f); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
+    template <typename P> __device__ __forceinline__ u32x4 piece(u32x4 q) const {
+        float d[P::N];
+        if (careful) {
+#pragma unroll
+            for (int j = 0; j < P::N; j++) d[j] = of(P::get(q, j));
+        } else {
+#pragma unroll
+            for (int j = 0; j < P::N; j++) d[j] = quick(P::get(q, j));
+        }
+        return P::put(d);
+    }
+    static __device__ __forceinline__ float action(const RowArgs& g, const RowNumbers& n) { return (n.c - exp_of(n.lpa) * (n.c + n.h * (n.lpa + n.H))) * g.inv_t; }
+};
+
 // G lanes take a row and hold it in registers, NV times 16 bytes each, from its one reading to the writing of the gradient.  What is over after the whole
 // 16-byte pieces (fewer than G values) goes to the first lanes, one value each.  MORE: the row may be longer than the registers; the pieces beyond are read in
 // batches, and for the gradient once more.  Workgroups stay for row after row; the rows of a pass over the grid are turned by `turn`, so that sequences padded at
@@ -223,7 +263,8 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
         const bool here = row < g.p.rows;
         auto one = [&](int i) -> float { return masked && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; };
         auto piece = [&](int c) -> u32x4 { u32x4 q = *(const u32x4_any*)(x + c * N); if (masked) q = P::forbid(q, P::bytes(mask + c * N)); return q; };
-        float logp = 0.f, H = 0.f, c = 0.f, h = 0.f, m = 0.f, L = 0.f, lpa = 0.f;
+        float m = 0.f;
+        RowNumbers n{};
         float xt = P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
         bool careful = false;
         if (on) {
@@ -273,28 +314,16 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
                 __syncthreads();
                 S = get_waves<G, Sum>(red[1]); Wt = get_waves<G, Sum>(red[2]);
             }
-            if (!(m > g.no_m)) on = S != S;               // nothing is allowed, but a NaN shows
-            if (on) {
-                L = __builtin_amdgcn_logf(S);            // (log2; S is about 1 at least)
-                H = LN2 * (L - Wt * __builtin_amdgcn_rcpf(S));
-                lpa = LN2 * (fmaf(xa, k, -m) - L);
-                H = H < 0.f ? 0.f : H;                                   // (the rounding of m can leave either an ulp of t off; a NaN stays)
-                lpa = lpa > 0.f ? 0.f : (lpa < -1e30f ? -1e30f : lpa);   // (-inf: below every floor, and 0 times it is wanted below)
-                const bool floored = lpa < g.log_floor;
-                logp = floored ? g.log_floor : lpa;
-                if (MODE == BACKWARD) { c = floored ? 0.f : g.d_logp[row]; h = g.d_entropy ? g.d_entropy[row] : 0.f; }
-                if (MODE == LOSS) {
-                    float st[STATS];
-                    loss_row(g, row, w, logp, H, floored, c, h, st);
-                    if (lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] += st[j];
-                }
-            }
+            float st[STATS];
+            n = row_numbers<MODE>(g, row, w, m, S, Wt, xa, st);
+            on = n.on;
+            if (MODE == LOSS && on && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] += st[j];
         }
         const bool ahead = AHEAD && counts(next_a, next_w);
         const T* next_x = logits(ahead ? next : 0);
         if (here && lane == 0) {
-            if (g.logp) g.logp[row] = logp;
-            if (g.entropy) g.entropy[row] = H;
+            if (g.logp) g.logp[row] = n.logp;
+            if (g.entropy) g.entropy[row] = n.H;
         }
         if (MODE == LOGP || !g.dlogits || !here || !on) {
             if (ahead) {
@@ -306,24 +335,10 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
                 if (lane < rest) dx[whole * N + lane] = (T)0.f;
             }
         } else {
-            // e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i); the action's own c / T comes in a store of its own behind it
-            const float inv = g.inv_t * __builtin_amdgcn_exp2f(-L), p1 = -h * LN2 * inv, p0 = -(c + h * (H - LN2 * L)) * inv;
-            auto grad = [&](float xv) -> float { const float t = fmaf(xv, k, -m); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); };
-            auto grad_careful = [&](float xv) -> float { const float t = fmaxf(fmaf(xv, k, -m), -1e30f); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); };
-            auto store = [&](char* to, u32x4 q) {
-                float d[N];
-                if (careful) {
-#pragma unroll
-                    for (int j = 0; j < N; j++) d[j] = grad_careful(P::get(q, j));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < N; j++) d[j] = grad(P::get(q, j));
-                }
-                *(u32x4_any*)to = P::put(d);
-            };
+            const RowGradient d(g, n, m, careful);
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                if (lane < whole - i * G) store((char*)dx + i * G * 16 + at, v[i]);
+                if (lane < whole - i * G) *(u32x4_any*)((char*)dx + i * G * 16 + at) = d.template piece<P>(v[i]);
                 if (ahead) fetch(next_x, i);
                 piece_done();
             }
@@ -333,12 +348,11 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
 #pragma unroll
                     for (int i = 0; i < BATCH; i++) if (p + i * G < whole) q[i] = piece(p + i * G);
 #pragma unroll
-                    for (int i = 0; i < BATCH; i++) { if (p + i * G < whole) store((char*)(dx + (p + i * G) * N), q[i]); piece_done(); }
+                    for (int i = 0; i < BATCH; i++) { if (p + i * G < whole) *(u32x4_any*)(dx + (p + i * G) * N) = d.template piece<P>(q[i]); piece_done(); }
                 }
-            if (lane < rest) dx[whole * N + lane] = (T)grad_careful(xt);
+            if (lane < rest) dx[whole * N + lane] = (T)d.of(xt);
             const int pa = a / N;
-            if (lane == (pa < whole ? pa % G : a - whole * N))
-                dx[a] = (T)((c - exp_of(lpa) * (c + h * (lpa + H))) * g.inv_t);       // its lane wrote the 16 bytes around it
+            if (lane == (pa < whole ? pa % G : a - whole * N)) dx[a] = (T)RowGradient::action(g, n);
         }
         row = next; a = next_a; w = next_w;
     }
@@ -349,6 +363,94 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
         for (int j = 1; j < RPB; j++) s += sums[j][threadIdx.x];
         g.row_stats[(int64_t)blockIdx.x * STATS + threadIdx.x] = s;
     }
+}
+
+// ---- few rows of many actions: a row over `splits` workgroups, `per` pieces each ---------------------------------------------------------------------------
+// k_parts leaves m, S and W of its part in part[row][split] and the action's logit behind the row's parts (the gradient may overwrite it before another part of
+// the row is done); k_join adds a row's parts up in every workgroup that needs them, in the same order, and writes the outputs and its part of the gradient.
+struct SplitArgs { int splits, per; float* part; };      // part: [rows][3 * splits + 1]
+template <typename T, Mode MODE> __device__ __forceinline__ bool row_counts(const RowArgs& g, int row, int& a, float& w) {
+    a = g.p.actions[row]; w = MODE == LOSS && g.loss.weights ? g.loss.weights[row] : 1.f;
+    return a >= 0 && a < g.p.n_actions && w != 0.f;
+}
+template <typename T> struct SplitRow {
+    using P = Pack<T>;
+    const T* x; const uint8_t* mask; bool masked; int whole, rest, from, to;
+    __device__ __forceinline__ SplitRow(const RowArgs& g, const SplitArgs& sp, int row, int split)
+        : x((const T*)g.p.logits + (int64_t)row * g.p.ld), mask(g.p.mask + (int64_t)row * g.p.ld_mask), masked(g.p.mask != nullptr), whole(g.p.n_actions / P::N),
+          rest(split == sp.splits - 1 ? g.p.n_actions - whole * P::N : 0), from(split * sp.per), to(min(whole, from + sp.per)) {}
+    __device__ __forceinline__ u32x4 piece(int c) const { u32x4 q = *(const u32x4_any*)(x + c * P::N); if (masked) q = P::forbid(q, P::bytes(mask + c * P::N)); return q; }
+    __device__ __forceinline__ float one(int i) const { return masked && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; }
+};
+template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(RowArgs g, SplitArgs sp) {
+    using P = Pack<T>;
+    __shared__ float red[3][4];
+    const int split = blockIdx.x, row = blockIdx.y, lane = threadIdx.x;
+    int a; float w;
+    if (!row_counts<T, MODE>(g, row, a, w)) return;       // (k_join does not look at it then)
+    const SplitRow<T> r(g, sp, row, split);
+    float* const part = sp.part + (int64_t)row * (3 * sp.splits + 1);
+    if (split == 0 && lane == 0) part[3 * sp.splits] = r.one(a);
+    const float xt = lane < r.rest ? r.one(r.whole * P::N + lane) : P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
+    RowSum s;
+    auto sum = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+        s.clear();
+        for (int p = r.from + lane; p < r.to; p += 4 * 256) {
+            u32x4 q[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { q[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; if (p + i * 256 < r.to) q[i] = r.piece(p + i * 256); }
+#pragma unroll
+            for (int i = 0; i < 4; i++) s.template piece<CAREFUL, P>(q[i], g.k);
+        }
+        s.reach(xt, g.k);
+        s.template add<CAREFUL>(xt, g.k, 1);
+    };
+    sum(std::false_type{});
+    float W = s.w[0] + s.w[1];
+    if (!(fabsf(W) < INFINITY)) { sum(std::true_type{}); W = s.w[0] + s.w[1]; }
+    float S = s.s[0] + s.s[1];
+    put_wave<256, Max>(s.m, red[0]);
+    __syncthreads();
+    const float m = get_waves<256, Max>(red[0]), by = s.m - m, f = __builtin_amdgcn_exp2f(by);
+    put_wave<256, Sum>(f * S, red[1]); put_wave<256, Sum>(f * fmaf(S, by, W), red[2]);
+    __syncthreads();
+    S = get_waves<256, Sum>(red[1]); W = get_waves<256, Sum>(red[2]);
+    if (lane == 0) { part[split] = m; part[sp.splits + split] = S; part[2 * sp.splits + split] = W; }
+}
+template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(RowArgs g, SplitArgs sp) {
+    using P = Pack<T>;
+    const int split = blockIdx.x, row = blockIdx.y, lane = threadIdx.x;
+    const SplitRow<T> r(g, sp, row, split);
+    int a; float w, m = NO_M;
+    RowNumbers n{};
+    float st[STATS] = {};
+    if (row_counts<T, MODE>(g, row, a, w)) {
+        const float* const part = sp.part + (int64_t)row * (3 * sp.splits + 1);
+        for (int i = lane & 63; i < sp.splits; i += 64) m = fmaxf(m, part[i]);
+        m = lanes<64, Max>(m);
+        float S = 0.f, W = 0.f;
+        for (int i = lane & 63; i < sp.splits; i += 64) {
+            const float by = part[i] - m, f = __builtin_amdgcn_exp2f(by), Si = part[sp.splits + i];
+            S += f * Si; W += f * fmaf(Si, by, part[2 * sp.splits + i]);
+        }
+        n = row_numbers<MODE>(g, row, w, m, lanes<64, Sum>(S), lanes<64, Sum>(W), part[3 * sp.splits], st);
+    }
+    if (split == 0) {
+        if (lane == 0) {
+            if (g.logp) g.logp[row] = n.logp;
+            if (g.entropy) g.entropy[row] = n.H;
+        }
+        if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) g.row_stats[row * STATS + j] = n.on ? st[j] : 0.f;
+    }
+    if (MODE == LOGP || !g.dlogits) return;
+    T* const dx = (T*)g.dlogits + (int64_t)row * g.ldd;
+    const RowGradient d(g, n, m, true);
+    for (int p = r.from + lane; p < r.to; p += 256) *(u32x4_any*)(dx + p * P::N) = n.on ? d.template piece<P>(r.piece(p)) : u32x4{0, 0, 0, 0};
+    if (lane < r.rest) dx[r.whole * P::N + lane] = (T)(n.on ? d.of(r.one(r.whole * P::N + lane)) : 0.f);
+    if (!n.on) return;
+    const int pa = a / P::N;
+    if (pa < r.whole ? pa >= r.from && pa < r.to && lane == (pa - r.from) % 256 : lane == a - r.whole * P::N && lane < r.rest) dx[a] = (T)RowGradient::action(g, n);
 }
 
 // The workgroups' statistics in a fixed order, in 64 bits: thread t adds the float4 t, t + 1024, ... (its four statistics of every 512th workgroup), the lanes of
@@ -495,9 +597,9 @@ struct OnDevice {
 int64_t size_of(int dtype) { return dtype == RLGPU_F32 ? 4 : (dtype == RLGPU_BF16 || dtype == RLGPU_F16 ? 2 : 0); }
 bool misaligned(const void* p, int64_t to) { return (uintptr_t)p % (uintptr_t)to != 0; }
 
-int64_t workspace_bytes_for(int rows) { return std::max<int64_t>(16, (int64_t)std::min(rows, ROW_BLOCKS) * STATS * 4); }
+int64_t policy_bytes(int dtype, int rows, int n_actions, bool loss);
 
-int check_rows(const char* who, const RlgpuPolicyRows* p, const void* workspace, int64_t bytes) {
+int check_rows(const char* who, const RlgpuPolicyRows* p, const void* workspace, int64_t bytes, bool loss = false) {
     if (!p) return fail(RLGPU_ERR_ARG, "%s: no rows", who);
     const int64_t size = size_of(p->dtype);
     if (!size) return fail(RLGPU_ERR_ARG, "%s: dtype %d is none of RLGPU_F32, RLGPU_BF16, RLGPU_F16", who, p->dtype);
@@ -506,18 +608,18 @@ int check_rows(const char* who, const RlgpuPolicyRows* p, const void* workspace,
     if (!(p->min_prob > 0.f && p->min_prob < 1.f)) return fail(RLGPU_ERR_ARG, "%s: min_prob %g is not between 0 and 1", who, (double)p->min_prob);
     if (p->rows == 0) return RLGPU_OK;
     if (!p->logits || !p->actions) return fail(RLGPU_ERR_ARG, "%s: logits and actions are needed", who);
-    if (p->rows > 1 && p->ld < p->n_actions) return fail(RLGPU_ERR_ARG, "%s: logits' row stride %lld is under %d actions", who, (long long)p->ld, p->n_actions);
-    if (p->mask && p->rows > 1 && p->ld_mask != 0 && p->ld_mask < p->n_actions) return fail(RLGPU_ERR_ARG, "%s: mask's row stride %lld", who, (long long)p->ld_mask);
+    if (p->rows > 1 && (p->ld < p->n_actions || p->ld > INT32_MAX)) return fail(RLGPU_ERR_ARG, "%s: logits' row stride %lld of %d actions", who, (long long)p->ld, p->n_actions);
+    if (p->mask && p->rows > 1 && p->ld_mask != 0 && (p->ld_mask < p->n_actions || p->ld_mask > INT32_MAX)) return fail(RLGPU_ERR_ARG, "%s: mask's row stride %lld", who, (long long)p->ld_mask);
     if (misaligned(p->logits, size) || misaligned(p->actions, 4)) return fail(RLGPU_ERR_ARG, "%s: logits or actions are not aligned to their type", who);
-    if (!workspace || misaligned(workspace, 16) || bytes < workspace_bytes_for(p->rows))
-        return fail(RLGPU_ERR_ARG, "%s: a workspace of %lld bytes, aligned to 16, is needed", who, (long long)workspace_bytes_for(p->rows));
+    const int64_t need = policy_bytes(p->dtype, p->rows, p->n_actions, loss);
+    if (need && (!workspace || misaligned(workspace, 16) || bytes < need)) return fail(RLGPU_ERR_ARG, "%s: a workspace of %lld bytes, aligned to 16, is needed", who, (long long)need);
     return RLGPU_OK;
 }
 // dlogits is the logits' own buffer, or shares no element with it: apart, or the other columns of the same rows
 int check_gradient(const char* who, const RlgpuPolicyRows* p, const void* dlogits, int64_t ldd) {
     if (!dlogits) return fail(RLGPU_ERR_ARG, "%s: dlogits is needed", who);
     const int64_t size = size_of(p->dtype), A = p->n_actions, R = p->rows;
-    if (R > 1 && ldd < A) return fail(RLGPU_ERR_ARG, "%s: dlogits' row stride %lld is under %lld actions", who, (long long)ldd, (long long)A);
+    if (R > 1 && (ldd < A || ldd > INT32_MAX)) return fail(RLGPU_ERR_ARG, "%s: dlogits' row stride %lld of %lld actions", who, (long long)ldd, (long long)A);
     if (misaligned(dlogits, size)) return fail(RLGPU_ERR_ARG, "%s: dlogits is not aligned to its type", who);
     const int64_t ld = R > 1 ? p->ld : A;
     if (R <= 1) ldd = A;
@@ -542,6 +644,27 @@ template <typename K> int resident(K kernel, int threads) {
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess) { (void)hipGetLastError(); per_cu = 1; }
     return std::max(1, std::min(ROW_BLOCKS, cus * per_cu));
 }
+// Few rows of many actions: a workgroup a row would leave the device idle.  Parts of at least a piece a lane, as many as give every CU two.
+constexpr int SPLIT_ROWS = 128, SPLIT_PIECES = 512, SPLIT_BLOCKS = 512;
+int splits_for(int dtype, int rows, int n_actions) {
+    const int whole = n_actions / (dtype == RLGPU_F32 ? 4 : 8);
+    if (rows == 0 || rows >= SPLIT_ROWS || whole <= SPLIT_PIECES) return 1;
+    return std::max(1, std::min((whole + 255) / 256, SPLIT_BLOCKS / rows));
+}
+int64_t stats_bytes(int rows) { return (int64_t)std::min(rows, ROW_BLOCKS) * STATS * 4; }
+template <typename T, Mode MODE> int launch_split(RowArgs& g, hipStream_t s, int splits, int& blocks) {
+    SplitArgs sp;
+    const int whole = g.p.n_actions / Pack<T>::N;
+    sp.per = (whole + splits - 1) / splits; sp.splits = (whole + sp.per - 1) / sp.per;
+    sp.part = (float*)((char*)g.row_stats + (MODE == LOSS ? stats_bytes(g.p.rows) : 0));
+    blocks = g.p.rows;
+    hipLaunchKernelGGL((k_parts<T, MODE>), dim3(sp.splits, g.p.rows), dim3(256), 0, s, g, sp);
+    OCHK(hipGetLastError());
+    const bool sums = MODE == LOGP || !g.dlogits;
+    hipLaunchKernelGGL((k_join<T, MODE>), dim3(sums ? 1 : sp.splits, g.p.rows), dim3(sums ? 64 : 256), 0, s, g, sp);
+    OCHK(hipGetLastError());
+    return RLGPU_OK;
+}
 template <typename T, int G, int NV, Mode MODE, bool MORE> int launch_rows_as(RowArgs& g, hipStream_t s, int& blocks) {
     constexpr int threads = G <= 64 ? 256 : G, rpb = threads / G;
     static const int most = resident(&k_rows<T, G, NV, MODE, MORE>, threads);
@@ -557,6 +680,8 @@ template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, in
     const uint32_t fill = Pack<T>::FILL; float low;
     if (sizeof(T) == 2 && fill == 0xfbfffbffu) low = -65504.f; else { const uint32_t f = fill & 0xffff0000u; std::memcpy(&low, &f, 4); }
     g.no_m = std::max(low * g.k, NO_M);
+    const int splits = splits_for(g.p.dtype, g.p.rows, g.p.n_actions);
+    if (splits > 1) return launch_split<T, MODE>(g, s, splits, blocks);
     if (whole <= 8) return launch_rows_as<T, 8, 1, MODE, false>(g, s, blocks);
     if (whole <= 8 * 2) return launch_rows_as<T, 8, 2, MODE, false>(g, s, blocks);
     if (whole <= 8 * 3) return launch_rows_as<T, 8, 3, MODE, false>(g, s, blocks);
@@ -582,6 +707,11 @@ template <Mode MODE> int launch_rows(const RowArgs& g, hipStream_t s, int& block
     return launch_rows_of<_Float16, MODE>(g, s, blocks);
 }
 
+int64_t policy_bytes(int dtype, int rows, int n_actions, bool loss) {
+    const int splits = splits_for(dtype, rows, n_actions);
+    return (loss ? stats_bytes(rows) : 0) + (splits > 1 ? (int64_t)rows * (3 * splits + 1) * 4 : 0);
+}
+
 int clip_batches(int n) { return std::max(1, (n + TENSORS - 1) / TENSORS); }
 int clip_share(int n_batches) { return std::max(256, 2 * CLIP_BLOCKS / n_batches); }   // workgroups of a launch, so that the partial sums stay few
 
@@ -591,9 +721,9 @@ extern "C" {
 
 const char* rlgpu_ops_last_error(void) { return g_error; }
 
-int64_t rlgpu_policy_workspace(int32_t dtype, int32_t rows, int32_t n_actions) {
-    if (!size_of(dtype) || rows < 0 || n_actions < 1) return fail(RLGPU_ERR_ARG, "rlgpu_policy_workspace: bad argument");
-    return workspace_bytes_for(rows);
+int64_t rlgpu_policy_workspace(int32_t dtype, int32_t rows, int32_t n_actions, int32_t loss) {
+    if (!size_of(dtype) || rows < 0 || n_actions < 1 || n_actions > (1 << 28)) return fail(RLGPU_ERR_ARG, "rlgpu_policy_workspace: bad argument");
+    return policy_bytes(dtype, rows, n_actions, loss != 0);
 }
 
 int rlgpu_action_logp(int device, const RlgpuPolicyRows* p, float* logp, float* entropy, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -602,7 +732,7 @@ int rlgpu_action_logp(int device, const RlgpuPolicyRows* p, float* logp, float* 
     if (!logp || misaligned(logp, 4) || misaligned(entropy, 4)) return fail(RLGPU_ERR_ARG, "rlgpu_action_logp: logp is needed, aligned to its type as entropy is");
     const OnDevice on(device); OCHK(on.err);
     RowArgs g = row_args(p);
-    g.logp = logp; g.entropy = entropy;
+    g.logp = logp; g.entropy = entropy; g.row_stats = (float*)workspace;
     int blocks;
     return launch_rows<LOGP>(g, (hipStream_t)stream, blocks);
 }
@@ -616,14 +746,14 @@ int rlgpu_action_logp_backward(int device, const RlgpuPolicyRows* p, const float
     if (int rc = check_gradient(who, p, dlogits, ld_dlogits)) return rc;
     const OnDevice on(device); OCHK(on.err);
     RowArgs g = row_args(p);
-    g.d_logp = d_logp; g.d_entropy = d_entropy; g.dlogits = dlogits; g.ldd = ld_dlogits;
+    g.d_logp = d_logp; g.d_entropy = d_entropy; g.dlogits = dlogits; g.ldd = ld_dlogits; g.row_stats = (float*)workspace;
     int blocks;
     return launch_rows<BACKWARD>(g, (hipStream_t)stream, blocks);
 }
 
 int rlgpu_policy_loss(int device, const RlgpuPolicyRows* p, const RlgpuPolicyLoss* l, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* who = "rlgpu_policy_loss";
-    if (int rc = check_rows(who, p, workspace, workspace_bytes)) return rc;
+    if (int rc = check_rows(who, p, workspace, workspace_bytes, true)) return rc;
     if (!l || !l->stats || misaligned(l->stats, 4)) return fail(RLGPU_ERR_ARG, "%s: the loss and its stats are needed", who);
     if (!(l->clip_low >= 0.f && l->clip_low < 1.f && l->clip_high >= 0.f && l->clip_high < INFINITY))
         return fail(RLGPU_ERR_ARG, "%s: clip range %g below and %g above 1", who, (double)l->clip_low, (double)l->clip_high);

@@ -201,6 +201,28 @@ def test_against_64_bits(A, dt, masked):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [1, 127, 128, 300])
+@pytest.mark.parametrize("A", [2500, 20011, 70001])
+def test_few_rows_and_many(A, rows):
+    """A row over several workgroups, or a workgroup a row: the same numbers, also where the gradient overwrites the logits."""
+    _, logits, actions, mask, g = make(rows, A, torch.bfloat16, seed=4, masked=True)
+    x, act, m = logits.cuda().contiguous(), actions.cuda(), mask.cuda()
+    r = ref_rows(logits, actions, mask)
+    logp, H = ops.action_logp(x, act, m)
+    check(logp, r["logp"], tol_logp(r, A), "logp")
+    check(H, r["H"], tol_entropy(r, A), "entropy")
+    dl, dh = torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+    zero = torch.zeros(rows, dtype=torch.float64)
+    c, h = torch.where(r["floored"] | ~r["on"], 0.0, dl.double()), torch.where(r["on"], dh.double(), 0.0)
+    want = ref_gradient(r, c, h, 1.0)
+    got = ops.action_logp_backward(x, act, dl.cuda(), dh.cuda(), m)
+    check(got, want, tol_gradient(r, c, h, zero, want, torch.bfloat16, 1.0), "dlogits")
+    for _ in range(3):
+        y = x.clone()
+        assert torch.equal(ops.action_logp_backward(y, act, dl.cuda(), dh.cuda(), m, out=y), got)
+
+
+@gpu
 @pytest.mark.parametrize("dt", list(DTYPES))
 @pytest.mark.parametrize("A", [6, 90, 700, 9001])
 def test_rows_with_nothing_to_learn(A, dt):
@@ -693,7 +715,7 @@ def test_refusals_of_the_library():
         return l
     N = 1 << 20
     bad_rows = [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(n_actions=0), dict(n_actions=(1 << 28) + 1), dict(temperature=0.0), dict(temperature=math.nan),
-                dict(temperature=1e-45), dict(min_prob=0.0), dict(min_prob=1.0), dict(logits=None), dict(actions=None), dict(ld=5), dict(mask=P, ld_mask=5),
+                dict(temperature=1e-45), dict(min_prob=0.0), dict(min_prob=1.0), dict(logits=None), dict(actions=None), dict(ld=5), dict(ld=1 << 31), dict(mask=P, ld_mask=5), dict(mask=P, ld_mask=1 << 31),
                 dict(logits=P + 2), dict(actions=P + 1), dict(dtype=1, logits=P + 1)]
     for kw in bad_rows:
         p = rows(**kw)
@@ -701,10 +723,13 @@ def test_refusals_of_the_library():
         assert lib.rlgpu_action_logp_backward(0, C.byref(p), P, None, 2 * P, 6, P, N, None) == -1
         assert lib.rlgpu_policy_loss(0, C.byref(p), C.byref(loss()), P, N, None) == -1
     p = rows()
-    need = lib.rlgpu_policy_workspace(0, 4, 6)
-    assert need > 0 and lib.rlgpu_policy_workspace(7, 4, 6) < 0 and lib.rlgpu_policy_workspace(0, -1, 6) < 0 and lib.rlgpu_policy_workspace(0, 4, 0) < 0
-    for ws, n in ((None, N), (P + 8, N), (P, need - 1)):
-        assert lib.rlgpu_action_logp(0, C.byref(p), P, None, ws, n, None) == -1
+    assert lib.rlgpu_policy_workspace(7, 4, 6, 0) < 0 and lib.rlgpu_policy_workspace(0, -1, 6, 0) < 0 and lib.rlgpu_policy_workspace(0, 4, 0, 1) < 0
+    assert lib.rlgpu_policy_workspace(0, 4, (1 << 28) + 1, 1) < 0 and lib.rlgpu_policy_workspace(0, 4, 6, 0) == 0
+    long = rows(n_actions=40000, ld=40000)                  # four rows of many actions: in parts
+    for ws, miss in ((None, 0), (P + 8, 0), (P, 1)):
+        assert lib.rlgpu_policy_loss(0, C.byref(p), C.byref(loss()), ws, lib.rlgpu_policy_workspace(0, 4, 6, 1) - miss, None) == -1
+        assert lib.rlgpu_action_logp(0, C.byref(long), P, None, ws, lib.rlgpu_policy_workspace(0, 4, 40000, 0) - miss, None) == -1
+        assert lib.rlgpu_action_logp_backward(0, C.byref(long), P, None, 2 * P, 40000, ws, lib.rlgpu_policy_workspace(0, 4, 40000, 0) - miss, None) == -1
     assert lib.rlgpu_action_logp(0, None, P, None, P, N, None) == -1
     assert lib.rlgpu_action_logp(0, C.byref(p), None, None, P, N, None) == -1
     for d, ld in ((None, 6), (2 * P, 5), (2 * P + 1, 6), (P + 4, 6), (P - 8, 6)):

@@ -22,6 +22,7 @@ namespace {
 
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
 constexpr int STATS = RLGPU_POLICY_STATS, ROW_BLOCKS = 2048;
+constexpr int64_t CACHE_BYTES = 256ll << 20, STREAM_BYTES = 2 * CACHE_BYTES;   // the last-level cache
 
 // what a launch over rows takes; mode decides which of the outputs are there
 struct RowArgs {
@@ -36,6 +37,7 @@ struct RowArgs {
     float* row_stats;                     // the workspace; the loss has [workgroups][STATS] in front: each workgroup's sums over its rows
 };
 enum Mode { LOGP, BACKWARD, LOSS };
+__device__ __forceinline__ int64_t row_offset(int row, int64_t ld) { return (int64_t)((uint64_t)(uint32_t)row * (uint32_t)ld); }   // (a stride has 32 bits, or there is one row)
 
 // e^x by the hardware's 2^x: off by an ulp and by the rounding of x log2(e), |x| 2^-24, which is what a difference of log-probabilities is off by already
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
@@ -117,6 +119,10 @@ template <> struct Pack<_Float16> : Pack16<_Float16, f16x2> {
     static __device__ __forceinline__ float get(u32x4 v, int j) { return (float)__builtin_bit_cast(f16x2, (uint32_t)v[j >> 1])[j & 1]; }
     static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xfbffu); }
 };
+
+// STREAM: past the caches.  Data of more than twice the last-level cache is gone from it before anybody asks again, and leaves there what others could use.
+template <bool STREAM> __device__ __forceinline__ u32x4 load(const void* p) { return STREAM ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p; }
+template <bool STREAM> __device__ __forceinline__ void store(void* p, u32x4 v) { if (STREAM) __builtin_nontemporal_store(v, (u32x4_any*)p); else *(u32x4_any*)p = v; }
 
 // The larger of three.  (fmaxf would first quiet each operand, an instruction a value; a NaN that is dropped here still makes the row's sum NaN.)
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c)); return r; }
@@ -227,7 +233,7 @@ struct RowGradient {
 // batches, and for the gradient once more.  Workgroups stay for row after row; the rows of a pass over the grid are turned by `turn`, so that sequences padded at
 // the same places do not leave some workgroups all the padding.  With 1024 lanes only one workgroup fits a CU, and it asks for its next row's pieces as it
 // writes the last's gradient: otherwise memory would wait for the sums and the sums for memory.
-template <typename T, int G, int NV, Mode MODE, bool MORE>
+template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM>
 __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
     using P = Pack<T>;
     constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = MODE == LOGP ? 4 : 2;
@@ -240,7 +246,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
     u32x4 v[NV];
     if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] = 0.f;   // (kept by the row's first lane)
     auto row_at = [&](int pass) { return (pass * (int)gridDim.x + (int)((blockIdx.x + (unsigned)pass * g.turn) % gridDim.x)) * RPB + sub; };
-    auto logits = [&](int row) { return (const T*)g.p.logits + (int64_t)row * g.p.ld; };
+    auto logits = [&](int row) { return (const T*)g.p.logits + row_offset(row, g.p.ld); };
     int row = row_at(0), a = -1; float w = 0.f;
     auto look = [&](int row, int& a, float& w) {          // a row beyond the last is left out
         a = -1; w = 0.f;
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
     auto counts = [&](int a, float w) { return a >= 0 && a < A && w != 0.f; };
     // piece i of the lane: a base that all lanes share (scalar registers) and one offset for all i
     const uint32_t at = (uint32_t)lane * 16u;
-    auto fetch = [&](const T* x, int i) { if (lane < whole - i * G) v[i] = *(const u32x4_any*)((const char*)x + i * G * 16 + at); };
+    auto fetch = [&](const T* x, int i) { if (lane < whole - i * G) v[i] = load<STREAM>((const char*)x + i * G * 16 + at); };
     look(row, a, w);
     for (int pass = 0; pass * (int)gridDim.x < groups; pass++) {
         const T* x = logits(row);
@@ -257,12 +263,12 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
         int next_a; float next_w;
         const bool last = (pass + 1) * (int)gridDim.x >= groups;
         if (last) { next_a = -1; next_w = 0.f; } else look(next, next_a, next_w);
-        const uint8_t* mask = g.p.mask + (int64_t)row * g.p.ld_mask;
-        T* dx = (T*)g.dlogits + (int64_t)row * g.ldd;
+        const uint8_t* mask = g.p.mask + row_offset(row, g.p.ld_mask);
+        T* dx = (T*)g.dlogits + row_offset(row, g.ldd);
         bool on = counts(a, w);
         const bool here = row < g.p.rows;
         auto one = [&](int i) -> float { return masked && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; };
-        auto piece = [&](int c) -> u32x4 { u32x4 q = *(const u32x4_any*)(x + c * N); if (masked) q = P::forbid(q, P::bytes(mask + c * N)); return q; };
+        auto piece = [&](int c) -> u32x4 { u32x4 q = load<STREAM>(x + c * N); if (masked) q = P::forbid(q, P::bytes(mask + c * N)); return q; };
         float m = 0.f;
         RowNumbers n{};
         float xt = P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
@@ -331,14 +337,14 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
                 for (int i = 0; i < NV; i++) { v[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; fetch(next_x, i); }
             }
             if (MODE != LOGP && g.dlogits && here) {
-                for (int p = lane; p < whole; p += G) *(u32x4_any*)(dx + p * N) = u32x4{0, 0, 0, 0};
+                for (int p = lane; p < whole; p += G) store<STREAM>(dx + p * N, u32x4{0, 0, 0, 0});
                 if (lane < rest) dx[whole * N + lane] = (T)0.f;
             }
         } else {
             const RowGradient d(g, n, m, careful);
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                if (lane < whole - i * G) *(u32x4_any*)((char*)dx + i * G * 16 + at) = d.template piece<P>(v[i]);
+                if (lane < whole - i * G) store<STREAM>((char*)dx + i * G * 16 + at, d.template piece<P>(v[i]));
                 if (ahead) fetch(next_x, i);
                 piece_done();
             }
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
 #pragma unroll
                     for (int i = 0; i < BATCH; i++) if (p + i * G < whole) q[i] = piece(p + i * G);
 #pragma unroll
-                    for (int i = 0; i < BATCH; i++) { if (p + i * G < whole) *(u32x4_any*)(dx + (p + i * G) * N) = d.template piece<P>(q[i]); piece_done(); }
+                    for (int i = 0; i < BATCH; i++) { if (p + i * G < whole) store<STREAM>(dx + (p + i * G) * N, d.template piece<P>(q[i])); piece_done(); }
                 }
             if (lane < rest) dx[whole * N + lane] = (T)d.of(xt);
             const int pa = a / N;
@@ -377,7 +383,7 @@ template <typename T> struct SplitRow {
     using P = Pack<T>;
     const T* x; const uint8_t* mask; bool masked; int whole, rest, from, to;
     __device__ __forceinline__ SplitRow(const RowArgs& g, const SplitArgs& sp, int row, int split)
-        : x((const T*)g.p.logits + (int64_t)row * g.p.ld), mask(g.p.mask + (int64_t)row * g.p.ld_mask), masked(g.p.mask != nullptr), whole(g.p.n_actions / P::N),
+        : x((const T*)g.p.logits + row_offset(row, g.p.ld)), mask(g.p.mask + row_offset(row, g.p.ld_mask)), masked(g.p.mask != nullptr), whole(g.p.n_actions / P::N),
           rest(split == sp.splits - 1 ? g.p.n_actions - whole * P::N : 0), from(split * sp.per), to(min(whole, from + sp.per)) {}
     __device__ __forceinline__ u32x4 piece(int c) const { u32x4 q = *(const u32x4_any*)(x + c * P::N); if (masked) q = P::forbid(q, P::bytes(mask + c * P::N)); return q; }
     __device__ __forceinline__ float one(int i) const { return masked && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; }
@@ -444,7 +450,7 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(R
         if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) g.row_stats[row * STATS + j] = n.on ? st[j] : 0.f;
     }
     if (MODE == LOGP || !g.dlogits) return;
-    T* const dx = (T*)g.dlogits + (int64_t)row * g.ldd;
+    T* const dx = (T*)g.dlogits + row_offset(row, g.ldd);
     const RowGradient d(g, n, m, true);
     for (int p = r.from + lane; p < r.to; p += 256) *(u32x4_any*)(dx + p * P::N) = n.on ? d.template piece<P>(r.piece(p)) : u32x4{0, 0, 0, 0};
     if (lane < r.rest) dx[r.whole * P::N + lane] = (T)(n.on ? d.of(r.one(r.whole * P::N + lane)) : 0.f);
@@ -496,18 +502,18 @@ template <typename F> __device__ __forceinline__ void for_pieces(const ClipBatch
         int lo = 0, hi = b.n;                                          // the last tensor whose first piece is <= piece (empty tensors share their successor's)
         while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (b.first[mid] <= piece) lo = mid; else hi = mid; }
         const int64_t at = (int64_t)(piece - b.first[lo]) * PIECE;
-        f(lo, at, (int)min((int64_t)PIECE, b.count[lo] - at));
+        f(piece, lo, at, (int)min((int64_t)PIECE, b.count[lo] - at));
     }
 }
 constexpr int IN_FLIGHT = 4;              // 16-byte loads of a lane
-template <typename T> __device__ __forceinline__ double square_sum(const T* g, int n) {
+template <bool STREAM, typename T> __device__ __forceinline__ double square_sum(const T* g, int n) {
     using P = Pack<T>;
     const int whole = n / P::N;
     double s[2] = {0, 0};
     for (int i = threadIdx.x; i < whole; i += IN_FLIGHT * 256) {
         u32x4 v[IN_FLIGHT];
 #pragma unroll
-        for (int j = 0; j < IN_FLIGHT; j++) { v[j] = u32x4{0, 0, 0, 0}; if (i + j * 256 < whole) v[j] = *(const u32x4_any*)(g + (i + j * 256) * P::N); }
+        for (int j = 0; j < IN_FLIGHT; j++) { v[j] = u32x4{0, 0, 0, 0}; if (i + j * 256 < whole) v[j] = load<STREAM>(g + (i + j * 256) * P::N); }
 #pragma unroll
         for (int j = 0; j < IN_FLIGHT; j++)
 #pragma unroll
@@ -524,14 +530,16 @@ __device__ __forceinline__ double block_sum(double s, double* red) {
     __syncthreads();
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
-__global__ void __launch_bounds__(256) k_grad_squares(ClipBatch b, double* part) {
+template <bool STREAM> __device__ __forceinline__ double squares_of(const ClipBatch& b, int t, int64_t at, int n) {
+    if (b.dtype[t] == RLGPU_F32) return square_sum<STREAM>((const float*)b.g[t] + at, n);
+    if (b.dtype[t] == RLGPU_BF16) return square_sum<STREAM>((const __bf16*)b.g[t] + at, n);
+    return square_sum<STREAM>((const _Float16*)b.g[t] + at, n);
+}
+// `stream`: so many of the first pieces are read past the caches, which is left to the last ones: the clip begins with those
+__global__ void __launch_bounds__(256) k_grad_squares(ClipBatch b, double* part, int stream) {
     __shared__ double red[4];
     double s = 0;
-    for_pieces(b, false, [&](int t, int64_t at, int n) {
-        if (b.dtype[t] == RLGPU_F32) s += square_sum((const float*)b.g[t] + at, n);
-        else if (b.dtype[t] == RLGPU_BF16) s += square_sum((const __bf16*)b.g[t] + at, n);
-        else s += square_sum((const _Float16*)b.g[t] + at, n);
-    });
+    for_pieces(b, false, [&](int piece, int t, int64_t at, int n) { s += piece < stream ? squares_of<true>(b, t, at, n) : squares_of<false>(b, t, at, n); });
     s = block_sum(s, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
@@ -563,7 +571,7 @@ __global__ void __launch_bounds__(256) k_grad_scale(ClipBatch b, const double* p
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const float f = (float)((double)grad_scale * fmin(1.0, (double)max_norm / (norm + 1e-6)));
     if (!(norm < INFINITY) || f == 1.f) return;
-    for_pieces(b, true, [&](int t, int64_t at, int n) {
+    for_pieces(b, true, [&](int, int t, int64_t at, int n) {
         if (b.dtype[t] == RLGPU_F32) scale_piece((float*)b.g[t] + at, n, f);
         else if (b.dtype[t] == RLGPU_BF16) scale_piece((__bf16*)b.g[t] + at, n, f);
         else scale_piece((_Float16*)b.g[t] + at, n, f);
@@ -665,12 +673,12 @@ template <typename T, Mode MODE> int launch_split(RowArgs& g, hipStream_t s, int
     OCHK(hipGetLastError());
     return RLGPU_OK;
 }
-template <typename T, int G, int NV, Mode MODE, bool MORE> int launch_rows_as(RowArgs& g, hipStream_t s, int& blocks) {
+template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM = false> int launch_rows_as(RowArgs& g, hipStream_t s, int& blocks) {
     constexpr int threads = G <= 64 ? 256 : G, rpb = threads / G;
-    static const int most = resident(&k_rows<T, G, NV, MODE, MORE>, threads);
+    static const int most = resident(&k_rows<T, G, NV, MODE, MORE, STREAM>, threads);
     blocks = std::min(most, (g.p.rows + rpb - 1) / rpb);
     g.turn = blocks * 5u / 13u;
-    hipLaunchKernelGGL((k_rows<T, G, NV, MODE, MORE>), dim3(blocks), dim3(threads), 0, s, g);
+    hipLaunchKernelGGL((k_rows<T, G, NV, MODE, MORE, STREAM>), dim3(blocks), dim3(threads), 0, s, g);
     OCHK(hipGetLastError());
     return RLGPU_OK;
 }
@@ -690,13 +698,14 @@ template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, in
     if (whole <= 64 * 2) return launch_rows_as<T, 64, 2, MODE, false>(g, s, blocks);
     if (whole <= 64 * 4) return launch_rows_as<T, 64, 4, MODE, false>(g, s, blocks);
     if (whole <= 64 * 8) return launch_rows_as<T, 64, 8, MODE, false>(g, s, blocks);
-    if constexpr (MODE == LOGP) return launch_rows_as<T, 256, 4, LOGP, true>(g, s, blocks);
+    const bool stream = (int64_t)g.p.rows * g.p.n_actions * (int64_t)sizeof(T) * (MODE != LOGP && g.dlogits ? 2 : 1) > STREAM_BYTES;
+    if constexpr (MODE == LOGP) return stream ? launch_rows_as<T, 256, 4, LOGP, true, true>(g, s, blocks) : launch_rows_as<T, 256, 4, LOGP, true>(g, s, blocks);
     else {
         if (whole <= 256 * 4) return launch_rows_as<T, 256, 4, MODE, false>(g, s, blocks);
         if (whole <= 256 * 8) return launch_rows_as<T, 256, 8, MODE, false>(g, s, blocks);
-        if (whole <= 1024 * 4) return launch_rows_as<T, 1024, 4, MODE, false>(g, s, blocks);
-        if (whole <= 1024 * 8) return launch_rows_as<T, 1024, 8, MODE, false>(g, s, blocks);
-        return launch_rows_as<T, 1024, 16, MODE, true>(g, s, blocks);
+        if (whole <= 1024 * 4) return stream ? launch_rows_as<T, 1024, 4, MODE, false, true>(g, s, blocks) : launch_rows_as<T, 1024, 4, MODE, false>(g, s, blocks);
+        if (whole <= 1024 * 8) return stream ? launch_rows_as<T, 1024, 8, MODE, false, true>(g, s, blocks) : launch_rows_as<T, 1024, 8, MODE, false>(g, s, blocks);
+        return stream ? launch_rows_as<T, 1024, 16, MODE, true, true>(g, s, blocks) : launch_rows_as<T, 1024, 16, MODE, true>(g, s, blocks);
     }
 }
 template <Mode MODE> int launch_rows(const RowArgs& g, hipStream_t s, int& blocks) {
@@ -824,11 +833,17 @@ int rlgpu_clip_grad_norm(int device, int32_t n, void* const* grads, const int64_
     };
     ClipBatch b;
     int n_part = 0;
+    int64_t to_stream = -CACHE_BYTES * 3 / 4;                          // bytes before those that shall be in the cache at the end
+    for (int i = 0; i < n; i++) to_stream += counts[i] * size_of(dtypes[i]);
     for (int k = 0; k < n_batches; k++) {
         const int blocks = batch(k, b);
         if (blocks < 0) return fail(RLGPU_ERR_ARG, "%s: too many elements", who);
         if (blocks == 0) continue;
-        hipLaunchKernelGGL(k_grad_squares, dim3(blocks), dim3(256), 0, s, b, part + n_part);
+        int64_t bytes = 0;
+        for (int i = 0; i < b.n; i++) bytes += b.count[i] * size_of(b.dtype[i]);
+        const int stream = to_stream <= 0 ? 0 : (int)std::min<double>(b.first[b.n], (double)to_stream / (double)bytes * b.first[b.n]);
+        to_stream -= bytes;
+        hipLaunchKernelGGL(k_grad_squares, dim3(blocks), dim3(256), 0, s, b, part + n_part, stream);
         OCHK(hipGetLastError());
         n_part += blocks;
     }

@@ -36,23 +36,24 @@ def _fail(rc):
 
 
 def _vector(name, t, rows, dtype, dev):
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != 1 or t.shape[0] != rows:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 1 and t.numel() == rows and t.is_contiguous() and t.device == dev:
+        return t.data_ptr()
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != 1 or t.numel() != rows:
         raise ValueError(f"{name}: a {str(dtype)[6:]} tensor of {rows} rows is needed")
-    if rows > 1 and t.stride(0) != 1:
-        raise ValueError(f"{name}: its rows have to be adjacent")
     if t.device != dev:
         raise ValueError(f"{name}: on {t.device}, the logits are on {dev}")
-    return t.data_ptr()
+    raise ValueError(f"{name}: its rows have to be adjacent")
 
 
 def _row_stride(name, t, rows, n):
-    if n > 1 and t.stride(1) != 1:
+    ld, one = t.stride()
+    if n > 1 and one != 1:
         raise ValueError(f"{name}: the actions of a row have to be adjacent")
-    return t.stride(0) if rows > 1 else n
+    return ld if rows > 1 else n
 
 
 def _rows(logits, actions, mask, temperature, min_prob):
-    """The RlgpuPolicyRows of a call, checked."""
+    """The RlgpuPolicyRows of a call, checked, its rows and its device."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise ValueError("logits: a float32, bfloat16 or float16 tensor [rows, n_actions] is needed")
     rows, n = logits.shape
@@ -63,31 +64,28 @@ def _rows(logits, actions, mask, temperature, min_prob):
     if not 0.0 < min_prob < 1.0:
         raise ValueError(f"min_prob: {min_prob} is not between 0 and 1")
     dev = logits.device
-    p = _lib.PolicyRows()
-    p.ld = _row_stride("logits", logits, rows, n)
-    if rows > 1 and p.ld < n:
+    ld = _row_stride("logits", logits, rows, n)
+    if rows > 1 and ld < n:
         raise ValueError("logits: its rows overlap (an expanded tensor)")
-    p.actions = _vector("actions", actions, rows, torch.int32, dev)
+    at = _vector("actions", actions, rows, torch.int32, dev)
+    mask_at, ld_mask = None, 0
     if mask is not None:
         if not isinstance(mask, torch.Tensor) or mask.dtype not in (torch.bool, torch.uint8) or mask.shape != logits.shape:
             raise ValueError(f"mask: a bool or uint8 tensor [{rows}, {n}] is needed (one row for all: mask.expand({rows}, {n}))")
         if mask.device != dev:
             raise ValueError(f"mask: on {mask.device}, the logits are on {dev}")
-        p.ld_mask = _row_stride("mask", mask, rows, n)
-        if rows > 1 and 0 < p.ld_mask < n:
+        ld_mask = _row_stride("mask", mask, rows, n)
+        if rows > 1 and 0 < ld_mask < n:
             raise ValueError("mask: its rows overlap")
-        p.mask = mask.data_ptr()
+        mask_at = mask.data_ptr()
     if dev.type != "cuda":
         raise ValueError("logits: the operators run on a GPU (there is no CPU path)")
-    p.logits = logits.data_ptr()
-    p.dtype = _DTYPES[logits.dtype]
-    p.rows, p.n_actions, p.temperature, p.min_prob = rows, n, temperature, min_prob
-    return p, dev
+    return _lib.PolicyRows(logits.data_ptr(), ld, mask_at, ld_mask, at, _DTYPES[logits.dtype], rows, n, temperature, min_prob), rows, dev
 
 
 def _gradient(out, logits):
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return torch.empty_like(logits, memory_format=torch.contiguous_format)
     if not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.dtype is not logits.dtype or out.device != logits.device:
         raise ValueError("out: a tensor of the logits' shape, type and device is needed")
     if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
@@ -95,11 +93,13 @@ def _gradient(out, logits):
     return out
 
 
-def _workspace(lib, p, dev, loss):
+def _workspace(lib, p, dev):
     """(the tensor to keep until the call has returned, its address, its bytes)"""
-    n = lib.rlgpu_policy_workspace(p.dtype, p.rows, p.n_actions, loss)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    return ws, ws.data_ptr() if n else None, n
+    n = lib.rlgpu_policy_workspace(p.dtype, p.rows, p.n_actions, 0)
+    if not n:
+        return None, None, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr(), n
 
 
 _stream = torch._C._cuda_getCurrentRawStream    # (device index) -> hipStream_t; torch.cuda.current_stream(device).cuda_stream without the object around it: 2 us less a call
@@ -108,11 +108,11 @@ _stream = torch._C._cuda_getCurrentRawStream    # (device index) -> hipStream_t;
 def action_logp(logits, actions, mask=None, *, temperature=1.0, min_prob=MIN_PROB):
     """(logp, entropy) per row: log max(softmax(logits / temperature)[action], min_prob) and the softmax's entropy over the actions that `mask` (True =
     allowed) lets through.  actions: int32; one outside [0, n_actions) leaves its row out, as a row in which nothing is allowed is: logp = entropy = 0."""
-    p, dev = _rows(logits, actions, mask, temperature, min_prob)
+    p, rows, dev = _rows(logits, actions, mask, temperature, min_prob)
     lib = _lib.load()
-    logp, entropy = torch.empty((2, p.rows), dtype=torch.float32, device=dev).unbind(0)
-    ws, ws_ptr, n = _workspace(lib, p, dev, 0)
-    rc = lib.rlgpu_action_logp(dev.index, C.byref(p), logp.data_ptr(), entropy.data_ptr(), ws_ptr, n, _stream(dev.index))
+    logp, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
+    ws, ws_at, n = _workspace(lib, p, dev)
+    rc = lib.rlgpu_action_logp(dev.index, C.byref(p), logp.data_ptr(), entropy.data_ptr(), ws_at, n, _stream(dev.index))
     if rc:
         _fail(rc)
     return logp, entropy
@@ -121,14 +121,14 @@ def action_logp(logits, actions, mask=None, *, temperature=1.0, min_prob=MIN_PRO
 def action_logp_backward(logits, actions, d_logp, d_entropy=None, mask=None, *, temperature=1.0, min_prob=MIN_PROB, out=None):
     """The gradient of sum(d_logp * logp + d_entropy * entropy) with respect to the logits, in the logits' type.  A logp at the floor passes none, rows left
     out and actions that are not allowed get 0.  out: where to write it; `logits` itself may be given."""
-    p, dev = _rows(logits, actions, mask, temperature, min_prob)
-    c = _vector("d_logp", d_logp, p.rows, torch.float32, dev)
-    h = _vector("d_entropy", d_entropy, p.rows, torch.float32, dev) if d_entropy is not None else None
+    p, rows, dev = _rows(logits, actions, mask, temperature, min_prob)
+    c = _vector("d_logp", d_logp, rows, torch.float32, dev)
+    h = _vector("d_entropy", d_entropy, rows, torch.float32, dev) if d_entropy is not None else None
     out = _gradient(out, logits)
-    ld = _row_stride("out", out, p.rows, p.n_actions)
+    ld = _row_stride("out", out, rows, logits.shape[1])
     lib = _lib.load()
-    ws, ws_ptr, n = _workspace(lib, p, dev, 0)
-    rc = lib.rlgpu_action_logp_backward(dev.index, C.byref(p), c, h, out.data_ptr(), ld, ws_ptr, n, _stream(dev.index))
+    ws, ws_at, n = _workspace(lib, p, dev)
+    rc = lib.rlgpu_action_logp_backward(dev.index, C.byref(p), c, h, out.data_ptr(), ld, ws_at, n, _stream(dev.index))
     if rc:
         _fail(rc)
     return out
@@ -140,32 +140,29 @@ def policy_loss(logits, actions, old_logp, adv, ref_logp=None, mask=None, weight
     r = exp(logp - old_logp), d = ref_logp - logp, and its gradient with respect to the logits, in one pass: a PolicyLoss.  clip_high defaults to
     clip_range.  A row with weight 0 is left out as in action_logp, and nothing else of it is looked at (padding may hold anything).  grad=False: no gradient.
     out: where to write the gradient; `logits` itself may be given."""
-    p, dev = _rows(logits, actions, mask, temperature, min_prob)
-    l = _lib.PolicyLossC()
-    l.old_logp = _vector("old_logp", old_logp, p.rows, torch.float32, dev)
-    l.adv = _vector("adv", adv, p.rows, torch.float32, dev)
-    if ref_logp is not None:
-        l.ref_logp = _vector("ref_logp", ref_logp, p.rows, torch.float32, dev)
-    elif kl_coef != 0.0:
+    p, rows, dev = _rows(logits, actions, mask, temperature, min_prob)
+    old_at, adv_at = _vector("old_logp", old_logp, rows, torch.float32, dev), _vector("adv", adv, rows, torch.float32, dev)
+    if ref_logp is None and kl_coef != 0.0:
         raise ValueError("kl_coef: needs ref_logp")
-    if weights is not None:
-        l.weights = _vector("weights", weights, p.rows, torch.float32, dev)
+    ref_at = _vector("ref_logp", ref_logp, rows, torch.float32, dev) if ref_logp is not None else None
+    weights_at = _vector("weights", weights, rows, torch.float32, dev) if weights is not None else None
     clip_high = clip_range if clip_high is None else clip_high
     if not 0.0 <= clip_range < 1.0 or not 0.0 <= clip_high < float("inf"):
         raise ValueError(f"clip range: {clip_range} below and {clip_high} above 1")
-    l.clip_low, l.clip_high, l.ent_coef, l.kl_coef, l.scale = clip_range, clip_high, ent_coef, kl_coef, scale
-    dlogits = None
+    dlogits, to, ld = None, None, 0
     if grad:
         dlogits = _gradient(out, logits)
-        l.dlogits, l.ld_dlogits = dlogits.data_ptr(), _row_stride("out", dlogits, p.rows, p.n_actions)
+        to, ld = dlogits.data_ptr(), _row_stride("out", dlogits, rows, logits.shape[1])
     elif out is not None:
         raise ValueError("out: without a gradient there is nothing to write")
     lib = _lib.load()
-    logp = torch.empty(p.rows, dtype=torch.float32, device=dev)
-    stats = torch.empty(8, dtype=torch.float32, device=dev)
-    l.logp, l.stats = logp.data_ptr(), stats.data_ptr()
-    ws, ws_ptr, n = _workspace(lib, p, dev, 1)
-    rc = lib.rlgpu_policy_loss(dev.index, C.byref(p), C.byref(l), ws_ptr, n, _stream(dev.index))
+    n = lib.rlgpu_policy_workspace(p.dtype, rows, p.n_actions, 1)
+    # one allocation: the workspace in front, then the statistics and the log-probabilities
+    buf = torch.empty(n // 4 + 8 + rows, dtype=torch.float32, device=dev)
+    _, stats, logp = buf.split_with_sizes((n // 4, 8, rows))
+    ws_at = buf.data_ptr()
+    l = _lib.PolicyLossC(old_at, adv_at, ref_at, weights_at, clip_range, clip_high, ent_coef, kl_coef, scale, ws_at + n + 32, ws_at + n, to, ld)
+    rc = lib.rlgpu_policy_loss(dev.index, C.byref(p), C.byref(l), ws_at, n, _stream(dev.index))
     if rc:
         _fail(rc)
     return PolicyLoss(stats, logp, dlogits)

@@ -47,17 +47,25 @@ __device__ __forceinline__ float exp_minus_1_minus(float x) {
     return fabsf(x) < 0.25f ? near : exp_of(x) - 1.f - x;
 }
 
+// what a row's numbers need besides its logits, asked for before the sums over them
+struct RowInputs { float w, u, v, ref; };                 // weight; d_logp and d_entropy, or old_logp and adv; ref_logp
+template <Mode MODE> __device__ __forceinline__ RowInputs row_inputs(const RowArgs& g, int row, float w) {
+    RowInputs r{w, 0.f, 0.f, 0.f};
+    if (MODE == BACKWARD) { r.u = g.d_logp[row]; r.v = g.d_entropy ? g.d_entropy[row] : 0.f; }
+    if (MODE == LOSS) { r.u = g.loss.old_logp[row]; r.v = g.loss.adv[row]; if (g.loss.ref_logp) r.ref = g.loss.ref_logp[row]; }
+    return r;
+}
 // one row of the loss: d loss / d logp and d loss / d entropy, and the row's part of the statistics
-__device__ void loss_row(const RowArgs& g, int row, float w, float logp, float H, bool floored, float& c, float& h, float (&st)[STATS]) {
+__device__ __forceinline__ void loss_row(const RowArgs& g, const RowInputs& in, float logp, float H, bool floored, float& c, float& h, float (&st)[STATS]) {
     const RlgpuPolicyLoss& l = g.loss;
-    const float x = logp - l.old_logp[row], adv = l.adv[row];
+    const float x = logp - in.u, adv = in.v, w = in.w;
     const float r = exp_of(x);
     const float surr = r * adv, clipped = fminf(fmaxf(r, 1.f - l.clip_low), 1.f + l.clip_high) * adv;
     float value = -(clipped < surr ? clipped : surr);     // (a NaN in either stays: surr holds it)
     c = clipped < surr ? 0.f : -surr;
     float ref = 0.f;
     if (l.ref_logp) {
-        const float d = l.ref_logp[row] - logp;
+        const float d = in.ref - logp;
         ref = exp_minus_1_minus(d);
         value += l.kl_coef * ref;
         c -= l.kl_coef * (ref + d);                       // exp(d) - 1
@@ -190,7 +198,7 @@ template <int G, typename OP> __device__ __forceinline__ float get_waves(const f
 
 // What follows from a row's m, S and W and its action's logit: whether it counts, its outputs, and what its gradient needs.
 struct RowNumbers { float logp, H, lpa, L, c, h; bool on; };
-template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const RowArgs& g, int row, float w, float m, float S, float W, float xa, float (&st)[STATS]) {
+template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const RowArgs& g, const RowInputs& in, float m, float S, float W, float xa, float (&st)[STATS]) {
     RowNumbers n{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, true};
     if (!(m > g.no_m)) n.on = S != S;                     // nothing is allowed, but a NaN shows
     if (!n.on) return n;
@@ -200,8 +208,8 @@ template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const Row
     n.lpa = lpa > 0.f ? 0.f : (lpa < -1e30f ? -1e30f : lpa);             // (-inf: below every floor, and 0 times it is wanted)
     const bool floored = n.lpa < g.log_floor;
     n.logp = floored ? g.log_floor : n.lpa;
-    if (MODE == BACKWARD) { n.c = floored ? 0.f : g.d_logp[row]; n.h = g.d_entropy ? g.d_entropy[row] : 0.f; }
-    if (MODE == LOSS) loss_row(g, row, w, n.logp, n.H, floored, n.c, n.h, st);
+    if (MODE == BACKWARD) { n.c = floored ? 0.f : in.u; n.h = in.v; }
+    if (MODE == LOSS) loss_row(g, in, n.logp, n.H, floored, n.c, n.h, st);
     return n;
 }
 // The gradient of a piece: e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i).  The action's own c / T comes in a store of its own, of the lane that
@@ -234,7 +242,7 @@ struct RowGradient {
 // the same places do not leave some workgroups all the padding.  With 1024 lanes only one workgroup fits a CU, and it asks for its next row's pieces as it
 // writes the last's gradient: otherwise memory would wait for the sums and the sums for memory.
 template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM>
-__global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
+__global__ void __launch_bounds__(G <= 64 ? 256 : G, G <= 16 ? 8 : 1) k_rows(RowArgs g) {
     using P = Pack<T>;
     constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = MODE == LOGP ? 4 : 2;
     constexpr bool AHEAD = G == 1024;
@@ -273,11 +281,13 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
         RowNumbers n{};
         float xt = P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
         bool careful = false;
-        if (on) {
-            if (!AHEAD || pass == 0) {
+        // (a short row is asked for before its action is known: two trips to memory would take longer than reading what is left out)
+        if ((!AHEAD || pass == 0) && (G <= 16 ? here : on)) {
 #pragma unroll
-                for (int i = 0; i < NV; i++) { v[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; fetch(x, i); }
-            }
+            for (int i = 0; i < NV; i++) { v[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; fetch(x, i); }
+        }
+        if (on) {
+            const RowInputs in = row_inputs<MODE>(g, row, w);
             if (lane < rest) xt = one(whole * N + lane);
             const float xa = one(a);
             if (masked) {
@@ -321,7 +331,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G) k_rows(RowArgs g) {
                 S = get_waves<G, Sum>(red[1]); Wt = get_waves<G, Sum>(red[2]);
             }
             float st[STATS];
-            n = row_numbers<MODE>(g, row, w, m, S, Wt, xa, st);
+            n = row_numbers<MODE>(g, in, m, S, Wt, xa, st);
             on = n.on;
             if (MODE == LOSS && on && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] += st[j];
         }
@@ -440,7 +450,7 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(R
             const float by = part[i] - m, f = __builtin_amdgcn_exp2f(by), Si = part[sp.splits + i];
             S += f * Si; W += f * fmaf(Si, by, part[2 * sp.splits + i]);
         }
-        n = row_numbers<MODE>(g, row, w, m, lanes<64, Sum>(S), lanes<64, Sum>(W), part[3 * sp.splits], st);
+        n = row_numbers<MODE>(g, row_inputs<MODE>(g, row, w), m, lanes<64, Sum>(S), lanes<64, Sum>(W), part[3 * sp.splits], st);
     }
     if (split == 0) {
         if (lane == 0) {
@@ -484,25 +494,27 @@ __global__ void __launch_bounds__(1024) k_row_stats(const float4* part, int n, f
 }
 
 // ---- gradient norm and clip ----------------------------------------------------------------------------------------------------------------------------
-// A launch takes up to TENSORS tensors by value, cut into pieces of PIECE elements; workgroup b takes the pieces b, b + gridDim.x, ...
-constexpr int TENSORS = 160, PIECE = 16384, CLIP_BLOCKS = 1024;
-struct ClipBatch {
-    int n;
+// A launch takes up to TENSORS tensors by value, cut into pieces; workgroup b takes the pieces b, b + gridDim.x, ...  A piece is PIECE elements where they fill the
+// device, SMALL_PIECE (two 16-byte loads a lane in float32) where they would not: the time is then one trip to memory.  A small network goes in a small batch:
+// 16 tensors take 28 us from the call to the end of the work with 0.6 KB of kernel arguments and 43 us with 3.8 KB (16.1 and 16.8 us a call in a row of calls).
+constexpr int TENSORS = 160, FEW_TENSORS = 24, PIECE = 16384, SMALL_PIECE = 2048, CLIP_BLOCKS = 1024;
+template <int TENSORS> struct ClipBatch {
+    int n, piece;                         // tensors, elements of a piece
     int first[TENSORS + 1];               // the first piece of each tensor; [n] = how many there are
     uint8_t dtype[TENSORS];
     void* g[TENSORS]; int64_t count[TENSORS];
 };
-static_assert(sizeof(ClipBatch) < 3900, "kernel arguments by value");
+static_assert(sizeof(ClipBatch<TENSORS>) < 3900, "kernel arguments by value");
 
 // `from_end`: the pieces in the opposite order.  The second reading of the gradients begins with what the first read last and the caches still hold.
-template <typename F> __device__ __forceinline__ void for_pieces(const ClipBatch& b, bool from_end, F&& f) {
+template <typename B, typename F> __device__ __forceinline__ void for_pieces(const B& b, bool from_end, F&& f) {
     const int n = b.first[b.n];
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
         const int piece = from_end ? n - 1 - i : i;
         int lo = 0, hi = b.n;                                          // the last tensor whose first piece is <= piece (empty tensors share their successor's)
         while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (b.first[mid] <= piece) lo = mid; else hi = mid; }
-        const int64_t at = (int64_t)(piece - b.first[lo]) * PIECE;
-        f(piece, lo, at, (int)min((int64_t)PIECE, b.count[lo] - at));
+        const int64_t at = (int64_t)(piece - b.first[lo]) * b.piece;
+        f(piece, lo, at, (int)min((int64_t)b.piece, b.count[lo] - at));
     }
 }
 constexpr int IN_FLIGHT = 4;              // 16-byte loads of a lane
@@ -530,13 +542,13 @@ __device__ __forceinline__ double block_sum(double s, double* red) {
     __syncthreads();
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
-template <bool STREAM> __device__ __forceinline__ double squares_of(const ClipBatch& b, int t, int64_t at, int n) {
+template <bool STREAM, typename B> __device__ __forceinline__ double squares_of(const B& b, int t, int64_t at, int n) {
     if (b.dtype[t] == RLGPU_F32) return square_sum<STREAM>((const float*)b.g[t] + at, n);
     if (b.dtype[t] == RLGPU_BF16) return square_sum<STREAM>((const __bf16*)b.g[t] + at, n);
     return square_sum<STREAM>((const _Float16*)b.g[t] + at, n);
 }
 // `stream`: so many of the first pieces are read past the caches, which is left to the last ones: the clip begins with those
-__global__ void __launch_bounds__(256) k_grad_squares(ClipBatch b, double* part, int stream) {
+template <typename B> __global__ void __launch_bounds__(256) k_grad_squares(B b, double* part, int stream) {
     __shared__ double red[4];
     double s = 0;
     for_pieces(b, false, [&](int piece, int t, int64_t at, int n) { s += piece < stream ? squares_of<true>(b, t, at, n) : squares_of<false>(b, t, at, n); });
@@ -562,10 +574,16 @@ template <typename T> __device__ __forceinline__ void scale_piece(T* g, int n, f
     if (i < n) g[i] = (T)((float)g[i] * f);
 }
 // every workgroup adds the partial sums up itself, all in the same order: no launch in between
-__global__ void __launch_bounds__(256) k_grad_scale(ClipBatch b, const double* part, int n_part, float max_norm, float grad_scale, float* norm_out) {
+template <typename B> __global__ void __launch_bounds__(256) k_grad_scale(B b, const double* part, int n_part, float max_norm, float grad_scale, float* norm_out) {
     __shared__ double red[4];
     double s = 0;
-    for (int i = threadIdx.x; i < n_part; i += 256) s += part[i];
+    for (int i = threadIdx.x; i < n_part; i += 8 * 256) {
+        double v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = i + j * 256 < n_part ? part[i + j * 256] : 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) s += v[j];
+    }
     s = block_sum(s, red);
     const double norm = (double)grad_scale * sqrt(s);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
@@ -724,6 +742,48 @@ int64_t policy_bytes(int dtype, int rows, int n_actions, bool loss) {
 int clip_batches(int n) { return std::max(1, (n + TENSORS - 1) / TENSORS); }
 int clip_share(int n_batches) { return std::max(256, 2 * CLIP_BLOCKS / n_batches); }   // workgroups of a launch, so that the partial sums stay few
 
+template <int TENSORS> int launch_clip(const char* who, int n, void* const* grads, const int64_t* counts, const int32_t* dtypes, bool writes, float max_norm, float grad_scale,
+                                       float* norm, double* part, hipStream_t s) {
+    const int n_batches = std::max(1, (n + TENSORS - 1) / TENSORS), share = clip_share(n_batches);
+    using Batch = ClipBatch<TENSORS>;
+    int64_t elements = 0, to_stream = -CACHE_BYTES * 3 / 4;            // (bytes before those that shall be in the cache at the end)
+    for (int i = 0; i < n; i++) { elements += counts[i]; to_stream += counts[i] * size_of(dtypes[i]); }
+    const int piece = elements < (int64_t)CLIP_BLOCKS * SMALL_PIECE ? SMALL_PIECE : PIECE;
+    auto batch = [&](int k, Batch& b) {                                // -> workgroups for it
+        int64_t pieces = 0;
+        b.piece = piece;
+        b.n = std::min(TENSORS, n - k * TENSORS);
+        for (int i = 0; i < b.n; i++) {
+            const int j = k * TENSORS + i;
+            b.g[i] = grads[j]; b.count[i] = counts[j]; b.dtype[i] = (uint8_t)dtypes[j]; b.first[i] = (int)pieces;
+            pieces += (counts[j] + piece - 1) / piece;
+        }
+        b.first[b.n] = (int)pieces;
+        return pieces > INT32_MAX ? -1 : (int)std::min<int64_t>(pieces, share);
+    };
+    Batch b;
+    int n_part = 0;
+    for (int k = 0; k < n_batches; k++) {
+        const int blocks = batch(k, b);
+        if (blocks < 0) return fail(RLGPU_ERR_ARG, "%s: too many elements", who);
+        if (blocks == 0) continue;
+        int64_t bytes = 0;
+        for (int i = 0; i < b.n; i++) bytes += b.count[i] * size_of(b.dtype[i]);
+        const int stream = to_stream <= 0 ? 0 : (int)std::min<double>(b.first[b.n], (double)to_stream / (double)bytes * b.first[b.n]);
+        to_stream -= bytes;
+        hipLaunchKernelGGL(k_grad_squares<Batch>, dim3(blocks), dim3(256), 0, s, b, part + n_part, stream);
+        OCHK(hipGetLastError());
+        n_part += blocks;
+    }
+    for (int k = n_batches - 1; k >= 0; k--) {
+        int blocks = writes ? (k == n_batches - 1 && k == 0 ? std::min(b.first[b.n], share) : batch(k, b)) : 0;
+        if (blocks == 0) { if (k) continue; b.n = 0; b.first[0] = 0; blocks = 1; }   // the last launch writes the norm, whatever there is to scale
+        hipLaunchKernelGGL(k_grad_scale<Batch>, dim3(blocks), dim3(256), 0, s, b, (const double*)part, n_part, max_norm, grad_scale, k == 0 ? norm : (float*)nullptr);
+        OCHK(hipGetLastError());
+    }
+    return RLGPU_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -817,43 +877,8 @@ int rlgpu_clip_grad_norm(int device, int32_t n, void* const* grads, const int64_
         }
     } catch (...) { return fail(RLGPU_ERR_NOMEM, "%s: out of host memory", who); }
     const OnDevice on(device); OCHK(on.err);
-    const hipStream_t s = (hipStream_t)stream;
-    double* const part = (double*)workspace;
-    const int n_batches = clip_batches(n), share = clip_share(n_batches);
-    auto batch = [&](int k, ClipBatch& b) {                            // -> workgroups for it
-        int64_t pieces = 0;
-        b.n = std::min(TENSORS, n - k * TENSORS);
-        for (int i = 0; i < b.n; i++) {
-            const int j = k * TENSORS + i;
-            b.g[i] = grads[j]; b.count[i] = counts[j]; b.dtype[i] = (uint8_t)dtypes[j]; b.first[i] = (int)pieces;
-            pieces += (counts[j] + PIECE - 1) / PIECE;
-        }
-        b.first[b.n] = (int)pieces;
-        return pieces > INT32_MAX ? -1 : (int)std::min<int64_t>(pieces, share);
-    };
-    ClipBatch b;
-    int n_part = 0;
-    int64_t to_stream = -CACHE_BYTES * 3 / 4;                          // bytes before those that shall be in the cache at the end
-    for (int i = 0; i < n; i++) to_stream += counts[i] * size_of(dtypes[i]);
-    for (int k = 0; k < n_batches; k++) {
-        const int blocks = batch(k, b);
-        if (blocks < 0) return fail(RLGPU_ERR_ARG, "%s: too many elements", who);
-        if (blocks == 0) continue;
-        int64_t bytes = 0;
-        for (int i = 0; i < b.n; i++) bytes += b.count[i] * size_of(b.dtype[i]);
-        const int stream = to_stream <= 0 ? 0 : (int)std::min<double>(b.first[b.n], (double)to_stream / (double)bytes * b.first[b.n]);
-        to_stream -= bytes;
-        hipLaunchKernelGGL(k_grad_squares, dim3(blocks), dim3(256), 0, s, b, part + n_part, stream);
-        OCHK(hipGetLastError());
-        n_part += blocks;
-    }
-    for (int k = n_batches - 1; k >= 0; k--) {
-        int blocks = writes ? batch(k, b) : 0;
-        if (blocks == 0) { if (k) continue; b.n = 0; b.first[0] = 0; blocks = 1; }   // the last launch writes the norm, whatever there is to scale
-        hipLaunchKernelGGL(k_grad_scale, dim3(blocks), dim3(256), 0, s, b, (const double*)part, n_part, max_norm, grad_scale, k == 0 ? norm : (float*)nullptr);
-        OCHK(hipGetLastError());
-    }
-    return RLGPU_OK;
+    const auto launch = n <= FEW_TENSORS ? launch_clip<FEW_TENSORS> : launch_clip<TENSORS>;
+    return launch(who, n, grads, counts, dtypes, writes, max_norm, grad_scale, norm, (double*)workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -28,7 +28,7 @@ constexpr int64_t CACHE_BYTES = 256ll << 20, STREAM_BYTES = 2 * CACHE_BYTES;   /
 struct RowArgs {
     RlgpuPolicyRows p;
     float k, inv_t, log_floor;            // log2(e) / T, 1 / T, log(min_prob)
-    float no_m;                           // a row whose m is no larger has nothing allowed
+    float none;                           // a row whose x0 is no larger has nothing allowed
     unsigned turn;
     float *logp, *entropy;                // optional
     const float *d_logp, *d_entropy;      // backward
@@ -67,8 +67,7 @@ __device__ __forceinline__ void loss_row(const RowArgs& g, const RowInputs& in, 
     if (l.ref_logp) {
         const float d = in.ref - logp;
         ref = exp_minus_1_minus(d);
-        value += l.kl_coef * ref;
-        c -= l.kl_coef * (ref + d);                       // exp(d) - 1
+        if (l.kl_coef != 0.f) { value += l.kl_coef * ref; c -= l.kl_coef * (ref + d); }      // (ref + d: exp(d) - 1)
     }
     value -= l.ent_coef * H;
     c = floored ? 0.f : c * w * l.scale;
@@ -139,38 +138,51 @@ __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm(
 // one pass for the next (219 registers where 32 hold a row in 16 bits, and spills in the largest).
 __device__ __forceinline__ void piece_done() { __builtin_amdgcn_sched_barrier(0); }
 
-// What a lane has of S and W.  `m` is the exponent (k x) that its sums are taken against: not the maximum, but within SLACK of it, so that it hardly ever moves
+// What a lane has of S and W.  `m` is the exponent (k x0) that its sums are taken against: not the maximum, but within SLACK of it, so that it hardly ever moves
 // after the first piece and a row is summed in one pass, piece by piece as it arrives.
-constexpr float SLACK = 8.f, NO_M = -1e38f;
+//
+// A quick sum can fail where logits are far from what a policy has: e t is NaN where t is -inf, and where k x passes FAR (the mask's FILL, a caller's -1e30) the
+// rounding of m would be an exponent itself.  W is then not finite, and the lane sums again with CAREFUL: against the exact maximum, with (x - x0) k for
+// k x - m where m is far, and no t below LOW.
+constexpr float SLACK = 8.f, FAR = 1e8f, LOWEST = -3.4028234663852886e38f;
+constexpr float LOW = -1e4f;              // 2^LOW is 0, and LOW times anything that occurs is finite: an exponent below is as good as LOW
+// k x0, rounded: left to itself the compiler joins the product with the difference that it is used in, and m would have another value in every place
+__device__ __forceinline__ float times_k(float x0, float k) {
+#pragma clang fp contract(off)
+    return x0 * k;
+}
+__device__ __forceinline__ bool is_far(float m) { return !(fabsf(m) < FAR); }
+__device__ __forceinline__ float exponent(float x, float k, float x0, float m) { return is_far(m) ? (x - x0) * k : fmaf(x, k, -m); }
+__device__ __forceinline__ float step_to(float x0, float m, float new_x0, float new_m, float k) { return fmaxf(is_far(m) || is_far(new_m) ? (x0 - new_x0) * k : m - new_m, LOW); }
 struct RowSum {
-    float m, s[2], w[2];
-    __device__ __forceinline__ void clear() { m = NO_M; s[0] = s[1] = w[0] = w[1] = 0.f; }
+    float x0, m, s[2], w[2];
+    __device__ __forceinline__ void clear() { x0 = LOWEST; m = -INFINITY; s[0] = s[1] = w[0] = w[1] = 0.f; }
+    __device__ __forceinline__ void start(float at, float k) { x0 = at; m = times_k(at, k); s[0] = s[1] = w[0] = w[1] = 0.f; }
     // `top`: the largest x of what comes next
-    __device__ __forceinline__ void reach(float top, float k) {
-        const float to = top * k;
-        if (to > m + SLACK) {
-            const bool fits = to < 3e38f;
-            const float by = m - (fits ? to : 0.f), f = __builtin_amdgcn_exp2f(by);
+    template <bool CAREFUL> __device__ __forceinline__ void reach(float top, float k) {
+        const float to = times_k(top, k);
+        if (CAREFUL ? top > x0 : to > m + SLACK) {
+            const float by = CAREFUL ? step_to(x0, m, top, to, k) : fmaxf(m - to, LOW), f = __builtin_amdgcn_exp2f(by);
             for (int j = 0; j < 2; j++) { w[j] = f * fmaf(s[j], by, w[j]); s[j] *= f; }
-            m = fits ? to : 0.f;
-            if (!fits) s[0] = NAN;                        // +inf among the logits
+            x0 = top; m = to;
         }
     }
-    // CAREFUL: some t may be -inf, and 0 times it is to be 0
     template <bool CAREFUL> __device__ __forceinline__ void add(float x, float k, int j) {
-        const float t = fmaf(x, k, -m), e = __builtin_amdgcn_exp2f(t);
-        s[j] += e; w[j] = fmaf(e, CAREFUL ? fmaxf(t, -1e30f) : t, w[j]);
+        const float t = CAREFUL ? exponent(x, k, x0, m) : fmaf(x, k, -m), e = __builtin_amdgcn_exp2f(t);
+        s[j] += e; w[j] = fmaf(e, CAREFUL ? fmaxf(t, LOW) : t, w[j]);
     }
     template <bool CAREFUL, typename P> __device__ __forceinline__ void piece(u32x4& v, float k) {
         float top = max3(P::get(v, 0), P::get(v, 1), P::get(v, 2));
 #pragma unroll
         for (int j = 3; j + 1 < P::N; j += 2) top = max3(top, P::get(v, j), P::get(v, j + 1));
-        reach(max3(top, P::get(v, P::N - 1), P::get(v, P::N - 1)), k);
+        reach<CAREFUL>(max3(top, P::get(v, P::N - 1), P::get(v, P::N - 1)), k);
 #pragma unroll
         for (int j = 0; j < P::N; j++) add<CAREFUL>(P::get(v, j), k, j & 1);
         asm("" : "+v"(v), "+v"(s[0]), "+v"(s[1]), "+v"(w[0]), "+v"(w[1]));
         piece_done();
     }
+    __device__ __forceinline__ float S() const { return s[0] + s[1]; }
+    __device__ __forceinline__ float W() const { return w[0] + w[1]; }
 };
 
 // ---- sums and maxima over the G lanes of a row; G <= 16 stays in a DPP row, more than 64 goes through LDS (`red`: one float a wavefront) ----------------------
@@ -196,16 +208,16 @@ template <int N, typename OP> __device__ __forceinline__ float lanes(float f) {
 template <int G, typename OP> __device__ __forceinline__ void put_wave(float v, float* red) { v = lanes<64, OP>(v); if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v; }
 template <int G, typename OP> __device__ __forceinline__ float get_waves(const float* red) { constexpr int W = G / 64; return lanes<W, OP>(red[threadIdx.x & (W - 1)]); }
 
-// What follows from a row's m, S and W and its action's logit: whether it counts, its outputs, and what its gradient needs.
+// What follows from a row's x0, S and W and its action's logit: whether it counts, its outputs, and what its gradient needs.
 struct RowNumbers { float logp, H, lpa, L, c, h; bool on; };
-template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const RowArgs& g, const RowInputs& in, float m, float S, float W, float xa, float (&st)[STATS]) {
+template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const RowArgs& g, const RowInputs& in, float x0, float S, float W, float xa, float (&st)[STATS]) {
     RowNumbers n{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, true};
-    if (!(m > g.no_m)) n.on = S != S;                     // nothing is allowed, but a NaN shows
+    if (!(x0 > g.none)) n.on = S != S;                    // nothing is allowed, but a NaN shows
     if (!n.on) return n;
     n.L = __builtin_amdgcn_logf(S);                       // (log2; S is about 1 at least)
-    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (fmaf(xa, g.k, -m) - n.L);
+    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (exponent(xa, g.k, x0, times_k(x0, g.k)) - n.L);
     n.H = H < 0.f ? 0.f : H;                              // (the rounding of m can leave either an ulp of t off; a NaN stays)
-    n.lpa = lpa > 0.f ? 0.f : (lpa < -1e30f ? -1e30f : lpa);             // (-inf: below every floor, and 0 times it is wanted)
+    n.lpa = lpa > 0.f ? 0.f : (lpa < LOW ? LOW : lpa);    // (below every floor)
     const bool floored = n.lpa < g.log_floor;
     n.logp = floored ? g.log_floor : n.lpa;
     if (MODE == BACKWARD) { n.c = floored ? 0.f : in.u; n.h = in.v; }
@@ -215,13 +227,14 @@ template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const Row
 // The gradient of a piece: e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i).  The action's own c / T comes in a store of its own, of the lane that
 // wrote the 16 bytes around it.
 struct RowGradient {
-    float k, m, p0, p1; bool careful;
-    __device__ __forceinline__ RowGradient(const RowArgs& g, const RowNumbers& n, float m, bool careful) : k(g.k), m(m), careful(careful) {
+    float k, x0, m, p0, p1; bool careful;
+    __device__ __forceinline__ RowGradient(const RowArgs& g, const RowNumbers& n, float x0, bool careful) : k(g.k), x0(x0), m(times_k(x0, g.k)) {
         const float inv = g.inv_t * __builtin_amdgcn_exp2f(-n.L);
         p1 = -n.h * LN2 * inv; p0 = -(n.c + n.h * (n.H - LN2 * n.L)) * inv;
+        this->careful = careful || is_far(m) || !(fabsf(p1) < 0.5f);   // an e_i of 0 times p1 t_i is 0 while that is finite: any t_i may be -3e38
     }
     __device__ __forceinline__ float quick(float x) const { const float t = fmaf(x, k, -m); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
-    __device__ __forceinline__ float of(float x) const { const float t = fmaxf(fmaf(x, k, -m), -1e30f); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
+    __device__ __forceinline__ float of(float x) const { const float t = fmaxf(exponent(x, k, x0, m), LOW); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
     template <typename P> __device__ __forceinline__ u32x4 piece(u32x4 q) const {
         float d[P::N];
         if (careful) {
@@ -242,9 +255,9 @@ struct RowGradient {
 // the same places do not leave some workgroups all the padding.  With 1024 lanes only one workgroup fits a CU, and it asks for its next row's pieces as it
 // writes the last's gradient: otherwise memory would wait for the sums and the sums for memory.
 template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM>
-__global__ void __launch_bounds__(G <= 64 ? 256 : G, G <= 16 ? 8 : 1) k_rows(RowArgs g) {
+__global__ void __launch_bounds__(G <= 64 ? 256 : G, MODE == BACKWARD && G <= 16 ? 8 : 1) k_rows(RowArgs g) {
     using P = Pack<T>;
-    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = MODE == LOGP ? 4 : 2;
+    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = 2;
     constexpr bool AHEAD = G == 1024;
     __shared__ float red[3][W], sums[RPB][STATS];
     const int lane = G <= 64 ? threadIdx.x % G : threadIdx.x, sub = G <= 64 ? threadIdx.x / G : 0;
@@ -277,7 +290,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G <= 16 ? 8 : 1) k_rows(Row
         const bool here = row < g.p.rows;
         auto one = [&](int i) -> float { return masked && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; };
         auto piece = [&](int c) -> u32x4 { u32x4 q = load<STREAM>(x + c * N); if (masked) q = P::forbid(q, P::bytes(mask + c * N)); return q; };
-        float m = 0.f;
+        float x0 = 0.f;
         RowNumbers n{};
         float xt = P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
         bool careful = false;
@@ -300,7 +313,6 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G <= 16 ? 8 : 1) k_rows(Row
             RowSum r;
             auto sum = [&](auto careful) {
                 constexpr bool CAREFUL = decltype(careful)::value;
-                r.clear();
 #pragma unroll
                 for (int i = 0; i < NV; i++) r.template piece<CAREFUL, P>(v[i], k);
                 if (MORE)
@@ -311,19 +323,23 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G <= 16 ? 8 : 1) k_rows(Row
 #pragma unroll
                         for (int i = 0; i < BATCH; i++) r.template piece<CAREFUL, P>(q[i], k);
                     }
-                r.reach(xt, k);
+                r.template reach<CAREFUL>(xt, k);
                 r.template add<CAREFUL>(xt, k, 1);
             };
+            r.clear();
             sum(std::false_type{});
-            float Wt = r.w[0] + r.w[1];
-            careful = !(fabsf(Wt) < INFINITY);
-            if (careful) { sum(std::true_type{}); Wt = r.w[0] + r.w[1]; }
-            float S = r.s[0] + r.s[1];
-            // the lanes' sums against the row's m
-            if (G <= 64) m = lanes<G, Max>(r.m);
-            else { put_wave<G, Max>(r.m, red[0]); __syncthreads(); m = get_waves<G, Max>(red[0]); }
-            const float by = r.m - m, f = __builtin_amdgcn_exp2f(by);
-            Wt = f * fmaf(S, by, Wt); S *= f;
+            careful = !(fabsf(r.W()) < INFINITY);
+            if (careful) { r.clear(); sum(std::true_type{}); }
+            // the lanes' sums against the row's x0
+            if (G <= 64) x0 = lanes<G, Max>(r.x0);
+            else { put_wave<G, Max>(r.x0, red[0]); __syncthreads(); x0 = get_waves<G, Max>(red[0]); }
+            const float m = times_k(x0, k);
+            float by;
+            if (is_far(m)) { r.start(x0, k); sum(std::true_type{}); by = step_to(r.x0, r.m, x0, m, k); }
+            else by = fmaxf(r.m - m, LOW);
+            const float f = __builtin_amdgcn_exp2f(by);
+            float S = r.S(), Wt = f * fmaf(S, by, r.W());
+            S *= f;
             if (G <= 64) { S = lanes<G, Sum>(S); Wt = lanes<G, Sum>(Wt); }
             else {
                 put_wave<G, Sum>(S, red[1]); put_wave<G, Sum>(Wt, red[2]);
@@ -331,7 +347,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G <= 16 ? 8 : 1) k_rows(Row
                 S = get_waves<G, Sum>(red[1]); Wt = get_waves<G, Sum>(red[2]);
             }
             float st[STATS];
-            n = row_numbers<MODE>(g, in, m, S, Wt, xa, st);
+            n = row_numbers<MODE>(g, in, x0, S, Wt, xa, st);
             on = n.on;
             if (MODE == LOSS && on && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] += st[j];
         }
@@ -351,7 +367,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G <= 16 ? 8 : 1) k_rows(Row
                 if (lane < rest) dx[whole * N + lane] = (T)0.f;
             }
         } else {
-            const RowGradient d(g, n, m, careful);
+            const RowGradient d(g, n, x0, careful);
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 if (lane < whole - i * G) store<STREAM>((char*)dx + i * G * 16 + at, d.template piece<P>(v[i]));
@@ -382,7 +398,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G <= 16 ? 8 : 1) k_rows(Row
 }
 
 // ---- few rows of many actions: a row over `splits` workgroups, `per` pieces each ---------------------------------------------------------------------------
-// k_parts leaves m, S and W of its part in part[row][split] and the action's logit behind the row's parts (the gradient may overwrite it before another part of
+// k_parts leaves x0, S and W of its part in part[row][split] and the action's logit behind the row's parts (the gradient may overwrite it before another part of
 // the row is done); k_join adds a row's parts up in every workgroup that needs them, in the same order, and writes the outputs and its part of the gradient.
 struct SplitArgs { int splits, per; float* part; };      // part: [rows][3 * splits + 1]
 template <typename T, Mode MODE> __device__ __forceinline__ bool row_counts(const RowArgs& g, int row, int& a, float& w) {
@@ -411,7 +427,6 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(
     RowSum s;
     auto sum = [&](auto careful) {
         constexpr bool CAREFUL = decltype(careful)::value;
-        s.clear();
         for (int p = r.from + lane; p < r.to; p += 4 * 256) {
             u32x4 q[4];
 #pragma unroll
@@ -419,38 +434,51 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(
 #pragma unroll
             for (int i = 0; i < 4; i++) s.template piece<CAREFUL, P>(q[i], g.k);
         }
-        s.reach(xt, g.k);
+        s.template reach<CAREFUL>(xt, g.k);
         s.template add<CAREFUL>(xt, g.k, 1);
     };
+    s.clear();
     sum(std::false_type{});
-    float W = s.w[0] + s.w[1];
-    if (!(fabsf(W) < INFINITY)) { sum(std::true_type{}); W = s.w[0] + s.w[1]; }
-    float S = s.s[0] + s.s[1];
-    put_wave<256, Max>(s.m, red[0]);
+    if (!(fabsf(s.W()) < INFINITY)) { s.clear(); sum(std::true_type{}); }
+    put_wave<256, Max>(s.x0, red[0]);
     __syncthreads();
-    const float m = get_waves<256, Max>(red[0]), by = s.m - m, f = __builtin_amdgcn_exp2f(by);
-    put_wave<256, Sum>(f * S, red[1]); put_wave<256, Sum>(f * fmaf(S, by, W), red[2]);
+    const float x0 = get_waves<256, Max>(red[0]);
+    const float m = times_k(x0, g.k);
+    float by;
+    if (is_far(m)) { s.start(x0, g.k); sum(std::true_type{}); by = step_to(s.x0, s.m, x0, m, g.k); }
+    else by = fmaxf(s.m - m, LOW);
+    const float f = __builtin_amdgcn_exp2f(by);
+    put_wave<256, Sum>(f * s.S(), red[1]); put_wave<256, Sum>(f * fmaf(s.S(), by, s.W()), red[2]);
     __syncthreads();
-    S = get_waves<256, Sum>(red[1]); W = get_waves<256, Sum>(red[2]);
-    if (lane == 0) { part[split] = m; part[sp.splits + split] = S; part[2 * sp.splits + split] = W; }
+    const float S = get_waves<256, Sum>(red[1]), W = get_waves<256, Sum>(red[2]);
+    if (lane == 0) { part[split] = x0; part[sp.splits + split] = S; part[2 * sp.splits + split] = W; }
 }
 template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(RowArgs g, SplitArgs sp) {
     using P = Pack<T>;
     const int split = blockIdx.x, row = blockIdx.y, lane = threadIdx.x;
     const SplitRow<T> r(g, sp, row, split);
-    int a; float w, m = NO_M;
+    int a; float w, x0 = LOWEST;
     RowNumbers n{};
     float st[STATS] = {};
+    // (the first pieces are asked for before the parts are joined)
+    constexpr int BATCH = 4;
+    const bool grad = MODE != LOGP && g.dlogits;
+    u32x4 q[BATCH];
+    auto fetch = [&](int p) {
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) if (p + i * 256 < r.to) q[i] = r.piece(p + i * 256);
+    };
+    if (grad) fetch(r.from + lane);
     if (row_counts<T, MODE>(g, row, a, w)) {
         const float* const part = sp.part + (int64_t)row * (3 * sp.splits + 1);
-        for (int i = lane & 63; i < sp.splits; i += 64) m = fmaxf(m, part[i]);
-        m = lanes<64, Max>(m);
+        for (int i = lane & 63; i < sp.splits; i += 64) x0 = fmaxf(x0, part[i]);
+        x0 = lanes<64, Max>(x0);
         float S = 0.f, W = 0.f;
         for (int i = lane & 63; i < sp.splits; i += 64) {
-            const float by = part[i] - m, f = __builtin_amdgcn_exp2f(by), Si = part[sp.splits + i];
+            const float by = step_to(part[i], times_k(part[i], g.k), x0, times_k(x0, g.k), g.k), f = __builtin_amdgcn_exp2f(by), Si = part[sp.splits + i];
             S += f * Si; W += f * fmaf(Si, by, part[2 * sp.splits + i]);
         }
-        n = row_numbers<MODE>(g, row_inputs<MODE>(g, row, w), m, lanes<64, Sum>(S), lanes<64, Sum>(W), part[3 * sp.splits], st);
+        n = row_numbers<MODE>(g, row_inputs<MODE>(g, row, w), x0, lanes<64, Sum>(S), lanes<64, Sum>(W), part[3 * sp.splits], st);
     }
     if (split == 0) {
         if (lane == 0) {
@@ -459,10 +487,14 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(R
         }
         if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) g.row_stats[row * STATS + j] = n.on ? st[j] : 0.f;
     }
-    if (MODE == LOGP || !g.dlogits) return;
+    if (!grad) return;
     T* const dx = (T*)g.dlogits + row_offset(row, g.ldd);
-    const RowGradient d(g, n, m, true);
-    for (int p = r.from + lane; p < r.to; p += 256) *(u32x4_any*)(dx + p * P::N) = n.on ? d.template piece<P>(r.piece(p)) : u32x4{0, 0, 0, 0};
+    const RowGradient d(g, n, x0, true);
+    for (int p = r.from + lane; p < r.to; p += BATCH * 256) {
+        if (p != r.from + lane) fetch(p);
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) if (p + i * 256 < r.to) store<false>(dx + (p + i * 256) * P::N, n.on ? d.template piece<P>(q[i]) : u32x4{0, 0, 0, 0});
+    }
     if (lane < r.rest) dx[r.whole * P::N + lane] = (T)(n.on ? d.of(r.one(r.whole * P::N + lane)) : 0.f);
     if (!n.on) return;
     const int pa = a / P::N;
@@ -517,7 +549,7 @@ template <typename B, typename F> __device__ __forceinline__ void for_pieces(con
         f(piece, lo, at, (int)min((int64_t)b.piece, b.count[lo] - at));
     }
 }
-constexpr int IN_FLIGHT = 4;              // 16-byte loads of a lane
+constexpr int IN_FLIGHT = 2;              // 16-byte loads of a lane
 template <bool STREAM, typename T> __device__ __forceinline__ double square_sum(const T* g, int n) {
     using P = Pack<T>;
     const int whole = n / P::N;
@@ -629,7 +661,7 @@ int check_rows(const char* who, const RlgpuPolicyRows* p, const void* workspace,
     if (!p) return fail(RLGPU_ERR_ARG, "%s: no rows", who);
     const int64_t size = size_of(p->dtype);
     if (!size) return fail(RLGPU_ERR_ARG, "%s: dtype %d is none of RLGPU_F32, RLGPU_BF16, RLGPU_F16", who, p->dtype);
-    if (p->rows < 0 || p->n_actions < 1 || p->n_actions > (1 << 28)) return fail(RLGPU_ERR_ARG, "%s: %d rows of %d actions", who, p->rows, p->n_actions);
+    if (p->rows < 0 || p->rows > (1 << 30) || p->n_actions < 1 || p->n_actions > (1 << 28)) return fail(RLGPU_ERR_ARG, "%s: %d rows of %d actions", who, p->rows, p->n_actions);
     if (!(p->temperature > 0.f) || !(p->temperature < INFINITY) || !(1.f / p->temperature < INFINITY)) return fail(RLGPU_ERR_ARG, "%s: temperature %g", who, (double)p->temperature);
     if (!(p->min_prob > 0.f && p->min_prob < 1.f)) return fail(RLGPU_ERR_ARG, "%s: min_prob %g is not between 0 and 1", who, (double)p->min_prob);
     if (p->rows == 0) return RLGPU_OK;
@@ -670,11 +702,13 @@ template <typename K> int resident(K kernel, int threads) {
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess) { (void)hipGetLastError(); per_cu = 1; }
     return std::max(1, std::min(ROW_BLOCKS, cus * per_cu));
 }
-// Few rows of many actions: a workgroup a row would leave the device idle.  Parts of at least a piece a lane, as many as give every CU two.
-constexpr int SPLIT_ROWS = 128, SPLIT_PIECES = 512, SPLIT_BLOCKS = 512;
+// Few rows of many actions: a workgroup a row would leave the device idle.  Parts of at least a piece a lane, as many as give every CU two.  Measured in parts
+// and as a workgroup a row, us for the backward pass in bfloat16: 131 072 actions 6.6 and 17.1 for 1 row, 8.9 and 18.2 for 32, 20.0 and 21.9 for 128, 34.4 and
+// 27.8 for 256; 20 000 actions (2 500 pieces) 6.2 and 5.7 for 1 row, 8.1 and 6.6 for 128.
+constexpr int SPLIT_ROWS = 128, SPLIT_PIECES = 4096, SPLIT_BLOCKS = 512;
 int splits_for(int dtype, int rows, int n_actions) {
     const int whole = n_actions / (dtype == RLGPU_F32 ? 4 : 8);
-    if (rows == 0 || rows >= SPLIT_ROWS || whole <= SPLIT_PIECES) return 1;
+    if (rows == 0 || rows > SPLIT_ROWS || whole <= SPLIT_PIECES) return 1;
     return std::max(1, std::min((whole + 255) / 256, SPLIT_BLOCKS / rows));
 }
 int64_t stats_bytes(int rows) { return (int64_t)std::min(rows, ROW_BLOCKS) * STATS * 4; }
@@ -705,7 +739,7 @@ template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, in
     const int whole = g.p.n_actions / Pack<T>::N;
     const uint32_t fill = Pack<T>::FILL; float low;
     if (sizeof(T) == 2 && fill == 0xfbfffbffu) low = -65504.f; else { const uint32_t f = fill & 0xffff0000u; std::memcpy(&low, &f, 4); }
-    g.no_m = std::max(low * g.k, NO_M);
+    g.none = low;
     const int splits = splits_for(g.p.dtype, g.p.rows, g.p.n_actions);
     if (splits > 1) return launch_split<T, MODE>(g, s, splits, blocks);
     if (whole <= 8) return launch_rows_as<T, 8, 1, MODE, false>(g, s, blocks);
@@ -717,7 +751,7 @@ template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, in
     if (whole <= 64 * 4) return launch_rows_as<T, 64, 4, MODE, false>(g, s, blocks);
     if (whole <= 64 * 8) return launch_rows_as<T, 64, 8, MODE, false>(g, s, blocks);
     const bool stream = (int64_t)g.p.rows * g.p.n_actions * (int64_t)sizeof(T) * (MODE != LOGP && g.dlogits ? 2 : 1) > STREAM_BYTES;
-    if constexpr (MODE == LOGP) return stream ? launch_rows_as<T, 256, 4, LOGP, true, true>(g, s, blocks) : launch_rows_as<T, 256, 4, LOGP, true>(g, s, blocks);
+    if constexpr (MODE == LOGP) return stream ? launch_rows_as<T, 256, 2, LOGP, true, true>(g, s, blocks) : launch_rows_as<T, 256, 2, LOGP, true>(g, s, blocks);
     else {
         if (whole <= 256 * 4) return launch_rows_as<T, 256, 4, MODE, false>(g, s, blocks);
         if (whole <= 256 * 8) return launch_rows_as<T, 256, 8, MODE, false>(g, s, blocks);
@@ -791,7 +825,7 @@ extern "C" {
 const char* rlgpu_ops_last_error(void) { return g_error; }
 
 int64_t rlgpu_policy_workspace(int32_t dtype, int32_t rows, int32_t n_actions, int32_t loss) {
-    if (!size_of(dtype) || rows < 0 || n_actions < 1 || n_actions > (1 << 28)) return fail(RLGPU_ERR_ARG, "rlgpu_policy_workspace: bad argument");
+    if (!size_of(dtype) || rows < 0 || rows > (1 << 30) || n_actions < 1 || n_actions > (1 << 28)) return fail(RLGPU_ERR_ARG, "rlgpu_policy_workspace: bad argument");
     return policy_bytes(dtype, rows, n_actions, loss != 0);
 }
 

@@ -57,7 +57,7 @@ def _rows(logits, actions, mask, temperature, min_prob):
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise ValueError("logits: a float32, bfloat16 or float16 tensor [rows, n_actions] is needed")
     rows, n = logits.shape
-    if n < 1 or n > 1 << 28 or rows >= 1 << 31:
+    if n < 1 or n > 1 << 28 or rows > 1 << 30:
         raise ValueError(f"logits: {rows} rows of {n} actions")
     if not 0.0 < temperature < float("inf"):
         raise ValueError(f"temperature: {temperature}")

@@ -101,7 +101,9 @@ def tol_gradient(r, c, h, dc, want, dtype, temperature):
     one[n, r["a"][r["on"]]] = 1
     size = c.abs()[:, None] * (one + s) + h.abs()[:, None] * s * (lp.abs().clamp(max=1e4) + r["H"][:, None] + 1)
     rel = U * (chain(A) + 32) + 2 * U * r["t"].abs().clamp(max=1e4)
+    # the hardware's 2^t is 0 where it would be under float32's smallest normal, 2^-126: that much of s, times what s is multiplied by
     tiny = 2.0 ** -25 if dtype is torch.float16 else 2.0 ** -126
+    tiny = tiny + 2.0 ** -126 * (c.abs()[:, None] + h.abs()[:, None] * (lp.abs().clamp(max=1e4) + r["H"][:, None] + 1)) / temperature
     return ((size * rel + dc[:, None] * (one + s)) / temperature) * (1 + half_step(dtype)) + half_step(dtype) * want.abs() + tiny
 
 
@@ -280,6 +282,68 @@ def test_rows_with_nothing_to_learn(A, dt):
 
 
 @gpu
+@pytest.mark.parametrize("how", ["mask", "lowest", "-inf", "-1e30", "-8e36"])
+@pytest.mark.parametrize("temperature", [0.01, 1.0, 2.0, 100.0])
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("A", [7, 90, 255, 1000, 9000, 140001])
+def test_all_but_a_few_masked(A, dt, temperature, how):
+    """Masks, by the mask or by the logits, that leave one to three actions anywhere in the row (most lanes have nothing), and coefficients far from 1."""
+    dtype = DTYPES[dt]
+    if dtype is torch.float16 and how in ("-1e30", "-8e36"):
+        how = "-inf"
+    R = 6
+    _, logits, _, _, g = make(R, A, dtype, seed=8, temperature=temperature)
+    keep = torch.zeros((R, A), dtype=torch.bool)
+    act = torch.randint(0, A, (R,), generator=g)
+    for i in range(R):
+        keep[i, act[i]] = True
+        keep[i, torch.randint(0, A, (i % 3,), generator=g)] = True
+    act = act.to(torch.int32)
+    x, mask = logits.clone(), None
+    if how == "mask":
+        x[~keep] = math.nan
+        mask = keep
+    else:
+        x[~keep] = {"lowest": torch.finfo(dtype).min, "-inf": -math.inf, "-1e30": -1e30, "-8e36": -8e36}[how]
+    r = ref_rows(torch.where(keep, logits, torch.zeros_like(logits)), act, keep, temperature)
+    m = None if mask is None else mask.cuda()
+    logp, H = ops.action_logp(x.cuda(), act.cuda(), m, temperature=temperature)
+    check(logp, r["logp"], tol_logp(r, A), "logp")
+    check(H, r["H"], tol_entropy(r, A), "entropy")
+    zero = torch.zeros(R, dtype=torch.float64)
+    for size in (1e-3, 1.0, 1e3):
+        c, h = torch.full((R,), 0.5 * size).double(), torch.full((R,), size).double()
+        if dtype is torch.float16:
+            c, h = c * min(1.0, temperature), h * min(1.0, temperature)        # (float16 holds 65504)
+        c, h = c.float().double(), h.float().double()
+        want = ref_gradient(r, torch.where(r["floored"], 0.0, c), h, temperature)
+        got = ops.action_logp_backward(x.cuda(), act.cuda(), c.float().cuda(), h.float().cuda(), m, temperature=temperature)
+        check(got, want, tol_gradient(r, c, h, zero, want, dtype, temperature), f"dlogits {size}")
+        assert (got[~keep.cuda()] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("base", [1e4, 1e6, 1e9, 1e30, -1e7, -1e9, -1e30])
+@pytest.mark.parametrize("temperature", [1e-4, 1.0])
+@pytest.mark.parametrize("A,rows", [(5, 9), (90, 9), (700, 9), (20000, 3), (20000, 200)])
+def test_far_logits(A, rows, temperature, base):
+    """Logits whose exponents are far from 0, spread over a few of float32's steps there."""
+    g = torch.Generator().manual_seed(A)
+    step = max(abs(base) * 2.0 ** -23, temperature)
+    x = (base + torch.randint(-4, 5, (rows, A), generator=g).double() * step).float()
+    act = x.argmax(1).to(torch.int32)
+    act[1] = x[1].argmin()
+    r = ref_rows(x, act, None, temperature)
+    logp, H = ops.action_logp(x.cuda(), act.cuda(), temperature=temperature)
+    check(logp, r["logp"], tol_logp(r, A), "logp")
+    check(H, r["H"], tol_entropy(r, A), "entropy")
+    c, h, zero = (torch.full((rows,), v).double() for v in (0.5, 0.25, 0.0))
+    want = ref_gradient(r, torch.where(r["floored"], 0.0, c), h, temperature)
+    got = ops.action_logp_backward(x.cuda(), act.cuda(), c.float().cuda(), h.float().cuda(), temperature=temperature)
+    check(got, want, tol_gradient(r, c, h, zero, want, torch.float32, temperature), "dlogits")
+
+
+@gpu
 @pytest.mark.parametrize("A", [5, 90, 3000])
 def test_nan_and_infinite_logits_show(A):
     x = torch.zeros((4, A))
@@ -327,6 +391,16 @@ def test_layouts(A, dt):
     # a vector of the batch that starts anywhere
     long = torch.randn(R + 3, generator=g).cuda(); long[2:2 + R] = dl
     assert torch.equal(ops.action_logp_backward(x, act, long[2:2 + R], dh, full), want)
+
+
+@gpu
+def test_a_reference_that_is_only_watched():
+    """kl_coef 0: the reference's log-probabilities are a statistic, whatever they are."""
+    x, a = torch.zeros((3, 5), device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    old, adv = torch.full((3,), -math.log(5.0), device="cuda"), torch.ones(3, device="cuda")
+    plain = ops.policy_loss(x, a, old, adv)
+    r = ops.policy_loss(x, a, old, adv, torch.tensor([-1.0, -math.inf, math.nan], device="cuda"))
+    assert torch.equal(r.dlogits, plain.dlogits) and r.stats[ops.STAT_LOSS] == plain.stats[ops.STAT_LOSS]
 
 
 @gpu
@@ -612,6 +686,14 @@ def test_graphs_streams_and_repetition(R, A, dt):
         got = everything(*sets[0])
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    # a size that no call has seen before the capture
+    fresh = torch.randn((5, 700 + R), device="cuda")
+    first = torch.zeros(5, dtype=torch.int32, device="cuda")
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        lp = ops.action_logp(fresh, first)[0]
+    gr.replay()
+    assert torch.equal(lp, ops.action_logp(fresh, first)[0])
     graphs, outs = [], []
     for s in sets:
         gr = torch.cuda.CUDAGraph()
@@ -714,7 +796,7 @@ def test_refusals_of_the_library():
             setattr(l, k, v)
         return l
     N = 1 << 20
-    bad_rows = [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(n_actions=0), dict(n_actions=(1 << 28) + 1), dict(temperature=0.0), dict(temperature=math.nan),
+    bad_rows = [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(rows=(1 << 30) + 1), dict(n_actions=0), dict(n_actions=(1 << 28) + 1), dict(temperature=0.0), dict(temperature=math.nan),
                 dict(temperature=1e-45), dict(min_prob=0.0), dict(min_prob=1.0), dict(logits=None), dict(actions=None), dict(ld=5), dict(ld=1 << 31), dict(mask=P, ld_mask=5), dict(mask=P, ld_mask=1 << 31),
                 dict(logits=P + 2), dict(actions=P + 1), dict(dtype=1, logits=P + 1)]
     for kw in bad_rows:

@@ -195,7 +195,8 @@ template <int N, typename OP> __device__ __forceinline__ int lanes_of(int v) {  
     if (N > 2) v = OP::of(v, dpp<0x4E>(v));               // quad_perm 2 3 0 1
     if (N > 4) v = OP::of(v, dpp<0x141>(v));              // row_half_mirror
     if (N > 8) v = OP::of(v, dpp<0x140>(v));              // row_mirror
-    if (N > 16) { v = OP::of(v, __shfl_xor(v, 16, 64)); v = OP::of(v, __shfl_xor(v, 32, 64)); }
+    if (N > 16) v = OP::of(v, __shfl_xor(v, 16, 64));
+    if (N > 32) v = OP::of(v, __shfl_xor(v, 32, 64));
     return v;
 }
 // floats as integers of the same order (their own inverse): maxima of integers need no quieting of NaN, which none of these is
@@ -255,9 +256,9 @@ struct RowGradient {
 // the same places do not leave some workgroups all the padding.  With 1024 lanes only one workgroup fits a CU, and it asks for its next row's pieces as it
 // writes the last's gradient: otherwise memory would wait for the sums and the sums for memory.
 template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM>
-__global__ void __launch_bounds__(G <= 64 ? 256 : G, MODE == BACKWARD && G <= 16 ? 8 : 1) k_rows(RowArgs g) {
+__global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACKWARD && G <= 16 ? 8 : 1) k_rows(RowArgs g) {
     using P = Pack<T>;
-    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = 2;
+    constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = MODE == LOGP ? 4 : 2;
     constexpr bool AHEAD = G == 1024;
     __shared__ float red[3][W], sums[RPB][STATS];
     const int lane = G <= 64 ? threadIdx.x % G : threadIdx.x, sub = G <= 64 ? threadIdx.x / G : 0;
@@ -747,16 +748,24 @@ template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, in
     if (whole <= 8 * 3) return launch_rows_as<T, 8, 3, MODE, false>(g, s, blocks);
     if (whole <= 8 * 4) return launch_rows_as<T, 8, 4, MODE, false>(g, s, blocks);
     if (whole <= 16 * 4) return launch_rows_as<T, 16, 4, MODE, false>(g, s, blocks);
-    if (whole <= 64 * 2) return launch_rows_as<T, 64, 2, MODE, false>(g, s, blocks);
+    if (whole <= 32 * 3) return launch_rows_as<T, 32, 3, MODE, false>(g, s, blocks);
+    if (whole <= 32 * 4) return launch_rows_as<T, 32, 4, MODE, false>(g, s, blocks);
+    if (whole <= 64 * 3) return launch_rows_as<T, 64, 3, MODE, false>(g, s, blocks);
     if (whole <= 64 * 4) return launch_rows_as<T, 64, 4, MODE, false>(g, s, blocks);
+    if (whole <= 64 * 6) return launch_rows_as<T, 64, 6, MODE, false>(g, s, blocks);
     if (whole <= 64 * 8) return launch_rows_as<T, 64, 8, MODE, false>(g, s, blocks);
+    if (whole <= 64 * 12) return launch_rows_as<T, 64, 12, MODE, false>(g, s, blocks);
+    if (whole <= 256 * 4) return launch_rows_as<T, 256, 4, MODE, false>(g, s, blocks);
     const bool stream = (int64_t)g.p.rows * g.p.n_actions * (int64_t)sizeof(T) * (MODE != LOGP && g.dlogits ? 2 : 1) > STREAM_BYTES;
     if constexpr (MODE == LOGP) return stream ? launch_rows_as<T, 256, 2, LOGP, true, true>(g, s, blocks) : launch_rows_as<T, 256, 2, LOGP, true>(g, s, blocks);
     else {
-        if (whole <= 256 * 4) return launch_rows_as<T, 256, 4, MODE, false>(g, s, blocks);
+        if (whole <= 256 * 6) return launch_rows_as<T, 256, 6, MODE, false>(g, s, blocks);
         if (whole <= 256 * 8) return launch_rows_as<T, 256, 8, MODE, false>(g, s, blocks);
-        if (whole <= 1024 * 4) return stream ? launch_rows_as<T, 1024, 4, MODE, false, true>(g, s, blocks) : launch_rows_as<T, 1024, 4, MODE, false>(g, s, blocks);
-        if (whole <= 1024 * 8) return stream ? launch_rows_as<T, 1024, 8, MODE, false, true>(g, s, blocks) : launch_rows_as<T, 1024, 8, MODE, false>(g, s, blocks);
+        if (whole <= 512 * 5) return launch_rows_as<T, 512, 5, MODE, false>(g, s, blocks);
+        if (whole <= 512 * 6) return launch_rows_as<T, 512, 6, MODE, false>(g, s, blocks);
+        if (whole <= 512 * 8) return launch_rows_as<T, 512, 8, MODE, false>(g, s, blocks);
+        if (whole <= 512 * 12) return stream ? launch_rows_as<T, 512, 12, MODE, false, true>(g, s, blocks) : launch_rows_as<T, 512, 12, MODE, false>(g, s, blocks);
+        if (whole <= 512 * 26) return stream ? launch_rows_as<T, 512, 16, MODE, true, true>(g, s, blocks) : launch_rows_as<T, 512, 16, MODE, true>(g, s, blocks);
         return stream ? launch_rows_as<T, 1024, 16, MODE, true, true>(g, s, blocks) : launch_rows_as<T, 1024, 16, MODE, true>(g, s, blocks);
     }
 }

@@ -202,8 +202,41 @@ def test_against_64_bits(A, dt, masked):
         assert alone.dlogits is None and torch.equal(alone.stats, got.stats) and torch.equal(alone.logp, got.logp)
 
 
+# the ends of the register sets a row may be held in (in 16-byte pieces): full, full with single values behind, and one piece more
+PIECES = [8, 16, 24, 32, 64, 96, 128, 192, 256, 384, 512, 768, 1024, 1536, 2048, 2560, 3072, 4096, 6144, 8192, 13312, 16384]
+
+
 @gpu
-@pytest.mark.parametrize("rows", [1, 127, 128, 300])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("pieces", PIECES)
+def test_ends_of_the_register_sets(pieces, dt, masked):
+    dtype = DTYPES[dt]
+    n = 4 if dt == "f32" else 8
+    for A in (pieces * n, pieces * n + n - 1, pieces * n + n):
+        rows = 131 if pieces > 4096 else 21               # (fewer rows of so many would be split)
+        _, logits, actions, mask, g = make(rows, A, dtype, seed=6, masked=masked)
+        x, act, m = logits.cuda(), actions.cuda(), None if mask is None else mask.cuda()
+        some = torch.tensor([0, 1, 2, 5, rows // 2, rows - 1])
+        r = ref_rows(logits[some], actions[some], None if mask is None else mask[some])
+        logp, H = ops.action_logp(x, act, m)
+        check(logp[some], r["logp"], tol_logp(r, A), f"logp {A}")
+        check(H[some], r["H"], tol_entropy(r, A), f"entropy {A}")
+        dl, dh = torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+        zero = torch.zeros(len(some), dtype=torch.float64)
+        c, h = torch.where(r["floored"] | ~r["on"], 0.0, dl[some].double()), torch.where(r["on"], dh[some].double(), 0.0)
+        want = ref_gradient(r, c, h, 1.0)
+        got = ops.action_logp_backward(x, act, dl.cuda(), dh.cuda(), m)
+        check(got[some], want, tol_gradient(r, c, h, zero, want, dtype, 1.0), f"dlogits {A}")
+        # the loss with old = logp: c = -adv r, the gradient of logp alone, and r = 1 but for what either logp is off by
+        loss = ops.policy_loss(x, act, logp, -dl.cuda(), None, m, clip_range=0.5)
+        want = ref_gradient(r, c, zero, 1.0)
+        check(loss.logp[some], r["logp"], tol_logp(r, A), f"loss: logp {A}")
+        check(loss.dlogits[some], want, tol_gradient(r, c, zero, c.abs() * (2 * tol_logp(r, A) + 8 * U), want, dtype, 1.0), f"loss: dlogits {A}")
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 127, 128, 129, 300])
 @pytest.mark.parametrize("A", [2500, 20011, 70001])
 def test_few_rows_and_many(A, rows):
     """A row over several workgroups, or a workgroup a row: the same numbers, also where the gradient overwrites the logits."""

@@ -389,14 +389,13 @@ typedef struct RlgpuPolicyRows {
     const void* logits; int64_t ld;           /* [rows][n_actions], row stride `ld` in elements (n_actions .. 2^31), any alignment of a row */
     const uint8_t* mask; int64_t ld_mask;     /* optional [rows][n_actions]: 0 = the action is not allowed, its logit is not looked at (it may be NaN); ld_mask 0: one row for all */
     const int32_t* actions;                   /* [rows]; an index outside 0 .. n_actions - 1 leaves the row out */
-    int32_t dtype, rows, n_actions;           /* RLGPU_F32 / BF16 / F16, rows >= 0, 1 <= n_actions <= 2^28 */
+    int32_t dtype, rows, n_actions;           /* RLGPU_F32 / BF16 / F16, 0 <= rows <= 2^30, 1 <= n_actions <= 2^28 */
     float temperature, min_prob;              /* > 0; the floor of a probability, 0 < min_prob < 1 (rlgpu_policy_act: 1e-11) */
 } RlgpuPolicyRows;
 /* Per row, over the allowed actions, with s = softmax(logits / temperature):
  *   logp = log max(s[action], min_prob)   (an action that is not allowed has s = 0),   entropy = -sum s log s   (0 log 0 = 0).
  * A row is LEFT OUT when its action is out of range or when nothing is allowed in it (mask all 0, or every allowed logit -inf or the type's lowest finite
- * value): logp = entropy = 0 and its gradient is zero.  NaN and +inf among the allowed logits give NaN.  Finite logits are taken within +-9e36 and
- * |logit| / temperature < 2e38; what is below counts as -inf, what is above as +inf.
+ * value, or below -9e36): logp = entropy = 0 and its gradient is zero.  NaN and +inf among the allowed logits of a row give NaN.
  * entropy may be NULL.  Workspace: rlgpu_policy_workspace bytes (0: it may be NULL), 16-byte aligned, free again when the call's work on the stream is done. */
 int64_t rlgpu_policy_workspace(int32_t dtype, int32_t rows, int32_t n_actions, int32_t loss /* 1: for rlgpu_policy_loss, 0: for the other two */);   /* bytes; < 0: bad argument */
 int rlgpu_action_logp(int device, const RlgpuPolicyRows* p, float* logp, float* entropy, void* workspace, int64_t workspace_bytes, void* hip_stream);

@@ -621,7 +621,7 @@ template <typename B> __global__ void __launch_bounds__(256) k_grad_scale(B b, c
     const double norm = (double)grad_scale * sqrt(s);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const float f = (float)((double)grad_scale * fmin(1.0, (double)max_norm / (norm + 1e-6)));
-    if (!(norm < INFINITY) || f == 1.f) return;
+    if (!(norm < INFINITY) || (grad_scale == 1.f && norm + 1e-6 <= (double)max_norm)) return;      // not a norm to clip by, or nothing to clip
     for_pieces(b, true, [&](int, int t, int64_t at, int n) {
         if (b.dtype[t] == RLGPU_F32) scale_piece((float*)b.g[t] + at, n, f);
         else if (b.dtype[t] == RLGPU_BF16) scale_piece((__bf16*)b.g[t] + at, n, f);

@@ -93,15 +93,6 @@ def _gradient(out, logits):
     return out
 
 
-def _workspace(lib, p, dev):
-    """(the tensor to keep until the call has returned, its address, its bytes)"""
-    n = lib.rlgpu_policy_workspace(p.dtype, p.rows, p.n_actions, 0)
-    if not n:
-        return None, None, 0
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    return ws, ws.data_ptr(), n
-
-
 _stream = torch._C._cuda_getCurrentRawStream    # (device index) -> hipStream_t; torch.cuda.current_stream(device).cuda_stream without the object around it: 2 us less a call
 
 
@@ -110,9 +101,12 @@ def action_logp(logits, actions, mask=None, *, temperature=1.0, min_prob=MIN_PRO
     allowed) lets through.  actions: int32; one outside [0, n_actions) leaves its row out, as a row in which nothing is allowed is: logp = entropy = 0."""
     p, rows, dev = _rows(logits, actions, mask, temperature, min_prob)
     lib = _lib.load()
-    logp, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
-    ws, ws_at, n = _workspace(lib, p, dev)
-    rc = lib.rlgpu_action_logp(dev.index, C.byref(p), logp.data_ptr(), entropy.data_ptr(), ws_at, n, _stream(dev.index))
+    n = lib.rlgpu_policy_workspace(p.dtype, rows, p.n_actions, 0)
+    # one allocation: the workspace in front (none for most sizes), then the outputs
+    buf = torch.empty(n // 4 + 2 * rows, dtype=torch.float32, device=dev)
+    _, logp, entropy = buf.split_with_sizes((n // 4, rows, rows))
+    at = buf.data_ptr()
+    rc = lib.rlgpu_action_logp(dev.index, C.byref(p), at + n, at + n + 4 * rows, at, n, _stream(dev.index))
     if rc:
         _fail(rc)
     return logp, entropy
@@ -127,8 +121,9 @@ def action_logp_backward(logits, actions, d_logp, d_entropy=None, mask=None, *, 
     out = _gradient(out, logits)
     ld = _row_stride("out", out, rows, logits.shape[1])
     lib = _lib.load()
-    ws, ws_at, n = _workspace(lib, p, dev)
-    rc = lib.rlgpu_action_logp_backward(dev.index, C.byref(p), c, h, out.data_ptr(), ld, ws_at, n, _stream(dev.index))
+    n = lib.rlgpu_policy_workspace(p.dtype, rows, p.n_actions, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    rc = lib.rlgpu_action_logp_backward(dev.index, C.byref(p), c, h, out.data_ptr(), ld, ws.data_ptr() if n else None, n, _stream(dev.index))
     if rc:
         _fail(rc)
     return out

@@ -252,9 +252,14 @@ def test_few_rows_and_many(A, rows):
     want = ref_gradient(r, c, h, 1.0)
     got = ops.action_logp_backward(x, act, dl.cuda(), dh.cuda(), m)
     check(got, want, tol_gradient(r, c, h, zero, want, torch.bfloat16, 1.0), "dlogits")
+    old, adv = torch.full((rows,), -5.0, device="cuda"), dl.cuda()
+    loss = ops.policy_loss(x, act, old, adv, None, m, ent_coef=0.01)
     for _ in range(3):
         y = x.clone()
         assert torch.equal(ops.action_logp_backward(y, act, dl.cuda(), dh.cuda(), m, out=y), got)
+        y = x.clone()
+        again = ops.policy_loss(y, act, old, adv, None, m, ent_coef=0.01, out=y)
+        assert torch.equal(y, loss.dlogits) and torch.equal(again.stats, loss.stats) and torch.equal(again.logp, loss.logp)
 
 
 @gpu
@@ -298,7 +303,9 @@ def test_rows_with_nothing_to_learn(A, dt):
     check(logp[keep], r["logp"][keep], tol_logp(r, A)[keep], "logp")
     check(H[keep], r["H"][keep], tol_entropy(r, A)[keep], "entropy")
     assert logp[10] == np.float32(FLOOR) and logp[11] == np.float32(FLOOR)
-    d = ops.action_logp_backward(c(x), c(act), c(torch.ones(R)), c(torch.full((R,), 0.5)), c(mask))
+    dl, dh = torch.ones(R), torch.full((R,), 0.5)
+    dl[:6] = dh[:6] = math.nan                              # (left out: whatever they are)
+    d = ops.action_logp_backward(c(x), c(act), c(dl), c(dh), c(mask))
     assert (d[left_out[:6] + [7]] == 0).all() and not d[keep].isnan().any()
     assert (d[9, 2:] == 0).all() and (d[10, 1] == 0)
     for kl in (0.0, 0.2):
@@ -312,6 +319,48 @@ def test_rows_with_nothing_to_learn(A, dt):
         dc = ww * (rho + kl * (torch.exp(dd) + 1)) * step
         check(got.dlogits, want, tol_gradient(rr, cc, hh, torch.where(rr["floored"], 0.0, dc), want, dtype, 1.0), "dlogits")
         check(got.stats[ops.STAT_LOSS], per_row[6].sum(), float((dc + 0.3 * tol_entropy(rr, A)).sum() + U * per_row[6].abs().sum()), "loss")
+
+
+@gpu
+@pytest.mark.parametrize("A,R,dt", [(5, 300001, "f32"), (90, 150001, "f32"), (250, 70001, "bf16"), (400, 50003, "bf16"), (700, 40001, "f16"), (1500, 30001, "bf16"), (5000, 9001, "bf16"),
+                                    (20000, 3001, "f32"), (40000, 4003, "bf16"), (70001, 4201, "f16"), (140001, 1301, "bf16"), (140001, 301, "f32")])
+def test_many_rows(A, R, dt):
+    """Workgroups that take row after row, padding and left-out rows among them, and calls that go past the caches: the same bits as in blocks of few rows, some
+    rows against 64 bits."""
+    dtype = DTYPES[dt]
+    g = torch.Generator(device="cuda").manual_seed(A)
+    x = (torch.randn((R, A), generator=g, device="cuda", dtype=torch.float32) * 2).to(dtype)
+    act = torch.randint(-1, A + 1, (R,), generator=g, device="cuda").to(torch.int32)        # a few out of range
+    act[::5] = x[::5].argmax(1).to(torch.int32)
+    at = torch.arange(R, device="cuda")
+    w = (at % 512 < torch.randint(1, 513, (R // 512 + 1,), generator=g, device="cuda")[at // 512]).float()
+    old, adv = torch.randn(R, generator=g, device="cuda") * 0.1 - 2, torch.randn(R, generator=g, device="cuda")
+    old[w == 0] = math.nan
+    dh = torch.randn(R, generator=g, device="cuda")
+
+    def calls(k, out=None):
+        lp, h = ops.action_logp(x[k], act[k])
+        d = ops.action_logp_backward(x[k], act[k], adv[k], dh[k])
+        r = ops.policy_loss(x[k], act[k], old[k], adv[k], None, None, w[k], ent_coef=0.01, scale=0.5)
+        return lp, h, d, r.logp, r.dlogits, r.stats
+    whole = calls(slice(0, R))
+    stats = torch.zeros(8, dtype=torch.float64, device="cuda")
+    step = max(129, min(3001, R // 3))
+    edges = list(range(0, R - 129, step)) + [R]                       # (blocks of more than 128 rows: fewer would be split)
+    for a, b in zip(edges, edges[1:]):
+        part = calls(slice(a, b))
+        for name, u, v in zip(("logp", "entropy", "backward", "loss logp", "loss dlogits"), whole, part):
+            assert torch.equal(u[a:b], v), f"{name}: rows {a} to {b}"
+        stats += part[5].double()
+    # each block's statistics are rounded once to float32, the workgroups' parts once a row
+    assert torch.allclose(whole[5].double(), stats, rtol=1e-5, atol=1e-5 * R)
+    assert whole[5][ops.STAT_ROWS] == ((act >= 0) & (act < A) & (w != 0)).sum()
+    some = torch.cat([torch.arange(4), torch.randint(0, R, (24,), generator=torch.Generator().manual_seed(1)), torch.arange(R - 4, R)])
+    r = ref_rows(x[some], act[some])
+    check(whole[0][some], r["logp"], tol_logp(r, A), "logp")
+    c, h = torch.where(r["floored"] | ~r["on"], 0.0, adv[some].double().cpu()), torch.where(r["on"], dh[some].double().cpu(), 0.0)
+    want = ref_gradient(r, c, h, 1.0)
+    check(whole[2][some], want, tol_gradient(r, c, h, 0 * c, want, dtype, 1.0), "dlogits")
 
 
 @gpu
@@ -631,10 +680,28 @@ def test_clip_sizes(counts, dt, scale):
     kinds = list(DTYPES.values()) if dt == "mixed" else [DTYPES[dt]]
     grads = [torch.randn(n, generator=g).to(kinds[i % len(kinds)]).cuda() for i, n in enumerate(counts)]
     total = math.sqrt(sum(counts))
-    check_clip([t.clone() for t in grads], 0.1 * total, scale)       # clipped
+    check_clip(list(t.clone() for t in grads), 0.1 * total, scale)       # clipped
     check_clip([t.clone() for t in grads], 10 * total + 1, scale)    # below
     check_clip([t.clone() for t in grads], math.inf, scale)
     check_clip([t.clone() for t in grads], 0.0, scale)
+
+
+@gpu
+def test_clip_many_tensors_and_a_large_one():
+    """More tensors than a few launches hold, in the order they come; a large one among them; one that is a generator's."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    grads = [torch.randn(1 + i % 7, generator=g, device="cuda").to(list(DTYPES.values())[i % 3]) for i in range(5003)]
+    grads.insert(2000, torch.randn(30_000_001, generator=g, device="cuda"))
+    grads.insert(4500, torch.randn(9_000_001, generator=g, device="cuda").bfloat16())
+    before = [t.clone() for t in grads]
+    exact = math.sqrt(sum(float((t.double() ** 2).sum()) for t in before))
+    n = ops.clip_grad_norm((t for t in grads), 1.0)
+    assert abs(float(n) - exact) <= 2 * U * exact
+    f = 1.0 / (exact + 1e-6)
+    for i in [0, 1, 2, 159, 160, 161, 1999, 2000, 2001, 4500, 5003, 5004]:
+        a, b = grads[i], before[i].double().cpu() * f
+        check(a, b, (half_step(a.dtype) + 4 * U) * b.abs() + 2.0 ** -25, "clipped")
+    assert all(torch.equal(a, (b.float() * f).to(a.dtype)) or (a.float() - b.float() * f).abs().max() <= 2 * half_step(a.dtype) * (b.float() * f).abs().max() + 2.0 ** -25 for a, b in zip(grads, before))
 
 
 @gpu

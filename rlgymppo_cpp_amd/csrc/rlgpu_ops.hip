@@ -588,7 +588,7 @@ template <typename B> __global__ void __launch_bounds__(256) k_grad_squares(B b,
     s = block_sum(s, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
-template <typename T> __device__ __forceinline__ void scale_piece(T* g, int n, float f) {
+template <typename T> __device__ __forceinline__ void scale_piece(T* g, int n, float f0, float f) {
     using P = Pack<T>;
     const int whole = n / P::N;
     for (int i = threadIdx.x; i < whole; i += IN_FLIGHT * 256) {
@@ -599,12 +599,12 @@ template <typename T> __device__ __forceinline__ void scale_piece(T* g, int n, f
         for (int j = 0; j < IN_FLIGHT; j++) {
             float d[P::N];
 #pragma unroll
-            for (int e = 0; e < P::N; e++) d[e] = P::get(v[j], e) * f;
+            for (int e = 0; e < P::N; e++) d[e] = P::get(v[j], e) * f0 * f;
             if (i + j * 256 < whole) *(u32x4_any*)(g + (i + j * 256) * P::N) = P::put(d);
         }
     }
     const int i = whole * P::N + threadIdx.x;
-    if (i < n) g[i] = (T)((float)g[i] * f);
+    if (i < n) g[i] = (T)((float)g[i] * f0 * f);
 }
 // every workgroup adds the partial sums up itself, all in the same order: no launch in between
 template <typename B> __global__ void __launch_bounds__(256) k_grad_scale(B b, const double* part, int n_part, float max_norm, float grad_scale, float* norm_out) {
@@ -620,12 +620,15 @@ template <typename B> __global__ void __launch_bounds__(256) k_grad_scale(B b, c
     s = block_sum(s, red);
     const double norm = (double)grad_scale * sqrt(s);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
-    const float f = (float)((double)grad_scale * fmin(1.0, (double)max_norm / (norm + 1e-6)));
-    if (!(norm < INFINITY) || (grad_scale == 1.f && norm + 1e-6 <= (double)max_norm)) return;      // not a norm to clip by, or nothing to clip
+    const double scale = (double)grad_scale * fmin(1.0, (double)max_norm / (norm + 1e-6));
+    // in two factors: gradients near float32's largest value are scaled by less than its smallest normal one (f0 is a power of two, and 1 elsewhere)
+    const float f0 = scale < 0x1p-100 ? 0x1p-64f : 1.f, f = (float)(scale < 0x1p-100 ? scale * 0x1p64 : scale);
+    // not a norm to clip by (as the caller sees it, in 32 bits), or nothing to clip
+    if (!((float)norm < INFINITY) || (grad_scale == 1.f && norm + 1e-6 <= (double)max_norm)) return;
     for_pieces(b, true, [&](int, int t, int64_t at, int n) {
-        if (b.dtype[t] == RLGPU_F32) scale_piece((float*)b.g[t] + at, n, f);
-        else if (b.dtype[t] == RLGPU_BF16) scale_piece((__bf16*)b.g[t] + at, n, f);
-        else scale_piece((_Float16*)b.g[t] + at, n, f);
+        if (b.dtype[t] == RLGPU_F32) scale_piece((float*)b.g[t] + at, n, f0, f);
+        else if (b.dtype[t] == RLGPU_BF16) scale_piece((__bf16*)b.g[t] + at, n, f0, f);
+        else scale_piece((_Float16*)b.g[t] + at, n, f0, f);
     });
 }
 

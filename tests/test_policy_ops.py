@@ -736,6 +736,16 @@ def test_clip_norm_that_is_not_finite():
 
 
 @gpu
+def test_clip_norm_past_float32():
+    """Finite gradients whose norm is inf as a float32: what the caller is told is not finite, so they stay; scaled into range they are clipped."""
+    for dtype in (torch.float32, torch.bfloat16):
+        a = torch.full((5,), 3e38, device="cuda").to(dtype)
+        keep = a.clone()
+        assert float(ops.clip_grad_norm([a], 0.5)) == math.inf and torch.equal(a, keep)
+        check_clip([a], 0.5, 2.0 ** -10)
+
+
+@gpu
 def test_clip_range_of_the_sum():
     """Squares that pass float32's range on both sides: the sum has 64 bits."""
     big = torch.full((1000,), 1e30, device="cuda")

@@ -21,7 +21,7 @@
 namespace {
 
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
-constexpr int STATS = RLGPU_POLICY_STATS, ROW_BLOCKS = 2048;
+constexpr int STATS = RLGPU_POLICY_STATS, ROW_BLOCKS = 2048, SPLIT_ROWS = 128;
 constexpr int64_t CACHE_BYTES = 256ll << 20, STREAM_BYTES = 2 * CACHE_BYTES;   // the last-level cache
 
 // what a launch over rows takes; mode decides which of the outputs are there
@@ -34,7 +34,7 @@ struct RowArgs {
     const float *d_logp, *d_entropy;      // backward
     RlgpuPolicyLoss loss;                 // loss
     void* dlogits; int64_t ldd;           // optional
-    float* row_stats;                     // the workspace; the loss has [workgroups][STATS] in front: each workgroup's sums over its rows
+    float* row_stats;                     // the workspace: of the loss [workgroups][STATS], each workgroup's sums over its rows; or a split call's parts
 };
 enum Mode { LOGP, BACKWARD, LOSS };
 __device__ __forceinline__ int64_t row_offset(int row, int64_t ld) { return (int64_t)((uint64_t)(uint32_t)row * (uint32_t)ld); }   // (a stride has 32 bits, or there is one row)
@@ -454,13 +454,53 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(
     const float S = get_waves<256, Sum>(red[1]), W = get_waves<256, Sum>(red[2]);
     if (lane == 0) { part[split] = x0; part[sp.splits + split] = S; part[2 * sp.splits + split] = W; }
 }
+// the parts of a row joined by `n` lanes, of which this is `at`
+__device__ __forceinline__ void join(const RowArgs& g, const SplitArgs& sp, const float* part, int at, int n, float& x0, float& S, float& W) {
+    x0 = LOWEST; S = W = 0.f;
+    for (int i = at; i < sp.splits; i += n) x0 = fmaxf(x0, part[i]);
+    for (int o = n >> 1; o > 0; o >>= 1) x0 = fmaxf(x0, __shfl_xor(x0, o, 64));
+    const float m = times_k(x0, g.k);
+    for (int i = at; i < sp.splits; i += n) {
+        const float by = step_to(part[i], times_k(part[i], g.k), x0, m, g.k), f = __builtin_amdgcn_exp2f(by), Si = part[sp.splits + i];
+        S += f * Si; W += f * fmaf(Si, by, part[2 * sp.splits + i]);
+    }
+    for (int o = n >> 1; o > 0; o >>= 1) { S += __shfl_xor(S, o, 64); W += __shfl_xor(W, o, 64); }
+}
+// The loss's statistics, by one workgroup beside those that write the gradient: 2 to 64 lanes a row, so that all rows are joined at once, then a sum over them in
+// 64 bits.  (A launch behind this one takes 3 us more, and 4 us more of the call.)
+template <typename T> __device__ __forceinline__ void split_stats(const RowArgs& g, const SplitArgs& sp) {
+    __shared__ float st[SPLIT_ROWS][STATS];
+    int n = 64;
+    while (n * g.p.rows > 256) n >>= 1;
+    const int row = threadIdx.x / n, at = threadIdx.x % n;
+    if (row < g.p.rows) {
+        float mine[STATS] = {}; bool on = false;
+        int a; float w;
+        if (row_counts<T, LOSS>(g, row, a, w)) {
+            const float* const part = sp.part + (int64_t)row * (3 * sp.splits + 1);
+            float x0, S, W;
+            join(g, sp, part, at, n, x0, S, W);
+            on = row_numbers<LOSS>(g, row_inputs<LOSS>(g, row, w), x0, S, W, part[3 * sp.splits], mine).on;
+        }
+        if (at == 0) for (int j = 0; j < STATS; j++) st[row][j] = on ? mine[j] : 0.f;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    double sum = 0;
+    for (int i = threadIdx.x / STATS; i < g.p.rows; i += 64 / STATS) sum += st[i][threadIdx.x % STATS];
+    for (int o = 32; o >= STATS; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (threadIdx.x < STATS) g.loss.stats[threadIdx.x] = (float)sum;
+}
 template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(RowArgs g, SplitArgs sp) {
     using P = Pack<T>;
     const int split = blockIdx.x, row = blockIdx.y, lane = threadIdx.x;
+    if (MODE == LOSS && split == (int)gridDim.x - 1) {    // (the loss has one workgroup more a row)
+        if (row == 0) split_stats<T>(g, sp);
+        return;
+    }
     const SplitRow<T> r(g, sp, row, split);
     int a; float w, x0 = LOWEST;
     RowNumbers n{};
-    float st[STATS] = {};
     // (the first pieces are asked for before the parts are joined)
     constexpr int BATCH = 4;
     const bool grad = MODE != LOGP && g.dlogits;
@@ -472,21 +512,13 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(R
     if (grad) fetch(r.from + lane);
     if (row_counts<T, MODE>(g, row, a, w)) {
         const float* const part = sp.part + (int64_t)row * (3 * sp.splits + 1);
-        for (int i = lane & 63; i < sp.splits; i += 64) x0 = fmaxf(x0, part[i]);
-        x0 = lanes<64, Max>(x0);
-        float S = 0.f, W = 0.f;
-        for (int i = lane & 63; i < sp.splits; i += 64) {
-            const float by = step_to(part[i], times_k(part[i], g.k), x0, times_k(x0, g.k), g.k), f = __builtin_amdgcn_exp2f(by), Si = part[sp.splits + i];
-            S += f * Si; W += f * fmaf(Si, by, part[2 * sp.splits + i]);
-        }
-        n = row_numbers<MODE>(g, row_inputs<MODE>(g, row, w), x0, lanes<64, Sum>(S), lanes<64, Sum>(W), part[3 * sp.splits], st);
+        float S, W, st[STATS];
+        join(g, sp, part, lane & 63, 64, x0, S, W);
+        n = row_numbers<MODE>(g, row_inputs<MODE>(g, row, w), x0, S, W, part[3 * sp.splits], st);
     }
-    if (split == 0) {
-        if (lane == 0) {
-            if (g.logp) g.logp[row] = n.logp;
-            if (g.entropy) g.entropy[row] = n.H;
-        }
-        if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) g.row_stats[row * STATS + j] = n.on ? st[j] : 0.f;
+    if (split == 0 && lane == 0) {
+        if (g.logp) g.logp[row] = n.logp;
+        if (g.entropy) g.entropy[row] = n.H;
     }
     if (!grad) return;
     T* const dx = (T*)g.dlogits + row_offset(row, g.ldd);
@@ -709,23 +741,24 @@ template <typename K> int resident(K kernel, int threads) {
 // Few rows of many actions: a workgroup a row would leave the device idle.  Parts of at least a piece a lane, as many as give every CU two.  Measured in parts
 // and as a workgroup a row, us for the backward pass in bfloat16: 131 072 actions 6.6 and 17.1 for 1 row, 8.9 and 18.2 for 32, 20.0 and 21.9 for 128, 34.4 and
 // 27.8 for 256; 20 000 actions (2 500 pieces) 6.2 and 5.7 for 1 row, 8.1 and 6.6 for 128.
-constexpr int SPLIT_ROWS = 128, SPLIT_PIECES = 4096, SPLIT_BLOCKS = 512;
+constexpr int SPLIT_PIECES = 4096, SPLIT_BLOCKS = 512;
 int splits_for(int dtype, int rows, int n_actions) {
     const int whole = n_actions / (dtype == RLGPU_F32 ? 4 : 8);
     if (rows == 0 || rows > SPLIT_ROWS || whole <= SPLIT_PIECES) return 1;
     return std::max(1, std::min((whole + 255) / 256, SPLIT_BLOCKS / rows));
 }
 int64_t stats_bytes(int rows) { return (int64_t)std::min(rows, ROW_BLOCKS) * STATS * 4; }
+constexpr int STATS_DONE = -1;            // (for `blocks`) there are no sums of workgroups to join
 template <typename T, Mode MODE> int launch_split(RowArgs& g, hipStream_t s, int splits, int& blocks) {
     SplitArgs sp;
     const int whole = g.p.n_actions / Pack<T>::N;
     sp.per = (whole + splits - 1) / splits; sp.splits = (whole + sp.per - 1) / sp.per;
-    sp.part = (float*)((char*)g.row_stats + (MODE == LOSS ? stats_bytes(g.p.rows) : 0));
-    blocks = g.p.rows;
+    sp.part = g.row_stats;
+    blocks = STATS_DONE;
     hipLaunchKernelGGL((k_parts<T, MODE>), dim3(sp.splits, g.p.rows), dim3(256), 0, s, g, sp);
     OCHK(hipGetLastError());
     const bool sums = MODE == LOGP || !g.dlogits;
-    hipLaunchKernelGGL((k_join<T, MODE>), dim3(sums ? 1 : sp.splits, g.p.rows), dim3(sums ? 64 : 256), 0, s, g, sp);
+    hipLaunchKernelGGL((k_join<T, MODE>), dim3((sums ? 1 : sp.splits) + (MODE == LOSS ? 1 : 0), g.p.rows), dim3(sums && MODE != LOSS ? 64 : 256), 0, s, g, sp);
     OCHK(hipGetLastError());
     return RLGPU_OK;
 }
@@ -783,7 +816,7 @@ template <Mode MODE> int launch_rows(const RowArgs& g, hipStream_t s, int& block
 
 int64_t policy_bytes(int dtype, int rows, int n_actions, bool loss) {
     const int splits = splits_for(dtype, rows, n_actions);
-    return (loss ? stats_bytes(rows) : 0) + (splits > 1 ? (int64_t)rows * (3 * splits + 1) * 4 : 0);
+    return splits > 1 ? (int64_t)rows * (3 * splits + 1) * 4 : (loss ? stats_bytes(rows) : 0);
 }
 
 int clip_batches(int n) { return std::max(1, (n + TENSORS - 1) / TENSORS); }
@@ -886,6 +919,7 @@ int rlgpu_policy_loss(int device, const RlgpuPolicyRows* p, const RlgpuPolicyLos
     g.loss = *l; g.logp = l->logp; g.dlogits = l->dlogits; g.ldd = l->ld_dlogits; g.row_stats = (float*)workspace;
     int blocks;
     if (int rc = launch_rows<LOSS>(g, (hipStream_t)stream, blocks)) return rc;
+    if (blocks == STATS_DONE) return RLGPU_OK;
     hipLaunchKernelGGL(k_row_stats, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const float4*)workspace, blocks, l->stats);
     OCHK(hipGetLastError());
     return RLGPU_OK;

@@ -383,7 +383,8 @@ const char* rlgpu_lt_last_error(void);
  * policy loss with a KL term with its gradient, the norm over all gradient tensors and the clip.  rlgpu_ppo_minibatch / rlgpu_clip_adam_step do the
  * same work inside the library's own MLPs.  There is no handle: every pointer is the caller's (device memory unless it says host), every launch goes to
  * `hip_stream` on `device`, nothing is kept between calls and nothing synchronises, so calls may be captured into graphs and may run at once on several
- * streams as long as each has a workspace of its own.  The text of an error: rlgpu_ops_last_error() (of the calling thread). */
+ * streams as long as each has a workspace of its own.  An output shares no memory with an input or with another output, except where it says so.  The text of
+ * an error: rlgpu_ops_last_error() (of the calling thread). */
 enum { RLGPU_F32 = 0, RLGPU_BF16 = 1, RLGPU_F16 = 2 };
 typedef struct RlgpuPolicyRows {
     const void* logits; int64_t ld;           /* [rows][n_actions], row stride `ld` in elements (n_actions .. 2^31), any alignment of a row */

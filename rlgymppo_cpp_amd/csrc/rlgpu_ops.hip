@@ -747,8 +747,8 @@ int splits_for(int dtype, int rows, int n_actions) {
     if (rows == 0 || rows > SPLIT_ROWS || whole <= SPLIT_PIECES) return 1;
     return std::max(1, std::min((whole + 255) / 256, SPLIT_BLOCKS / rows));
 }
-int64_t stats_bytes(int rows) { return (int64_t)std::min(rows, ROW_BLOCKS) * STATS * 4; }
 constexpr int STATS_DONE = -1;            // (for `blocks`) there are no sums of workgroups to join
+int64_t stats_bytes(int rows) { return (int64_t)std::min(rows, ROW_BLOCKS) * STATS * 4; }
 template <typename T, Mode MODE> int launch_split(RowArgs& g, hipStream_t s, int splits, int& blocks) {
     SplitArgs sp;
     const int whole = g.p.n_actions / Pack<T>::N;
@@ -768,8 +768,11 @@ template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM = false> 
     const int groups = (g.p.rows + rpb - 1) / rpb, passes = (groups + most - 1) / most;
     blocks = (groups + passes - 1) / passes;              // as many rows for each (2 048 groups: 1 024 workgroups twice, 12.1 us, not 1 536 and then 512, 12.5)
     g.turn = blocks * 5u / 13u;
+    const bool alone = MODE == LOSS && blocks == 1;       // its sums are the statistics
+    if (alone) g.row_stats = g.loss.stats;
     hipLaunchKernelGGL((k_rows<T, G, NV, MODE, MORE, STREAM>), dim3(blocks), dim3(threads), 0, s, g);
     OCHK(hipGetLastError());
+    if (alone) blocks = STATS_DONE;
     return RLGPU_OK;
 }
 // Lanes and 16-byte pieces a row: the smallest set of registers that holds it.  Sums alone need no more of a row than what is in flight: 256 lanes take any.

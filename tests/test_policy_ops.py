@@ -263,6 +263,36 @@ def test_few_rows_and_many(A, rows):
 
 
 @gpu
+@pytest.mark.parametrize("A,dt,rows", [(33001, "bf16", r) for r in (1, 2, 3, 5, 31, 64, 65, 127, 128, 129)] + [(17001, "f32", 6), (90, "f32", 1), (90, "f32", 32), (90, "f32", 33),
+                                       (700, "f16", 3), (2000, "bf16", 4), (9000, "f32", 1)])
+def test_statistics_of_few_rows(A, dt, rows):
+    """The sums over the rows wherever they are formed: one workgroup, a row over several, more of both; rows that do not count are among them."""
+    _, logits, actions, mask, g = make(rows, A, DTYPES[dt], seed=rows, masked=True)
+    w = torch.rand(rows, generator=g) + 0.5
+    w[2::5] = 0.0
+    actions[3::7] = -1
+    mask[4::9] = False
+    first = ref_rows(logits, actions, mask)
+    old, adv, ref = loss_inputs(rows, g, first["logp"])
+    old[2::5] = math.nan                                    # (weight 0: nothing else is looked at)
+    clean = torch.where(w == 0, torch.zeros_like(old), old)
+    r, rho, d, ww, c, h, per_row = ref_loss(logits, actions, clean, adv, ref, mask, w, ent=0.01, kl=0.1, scale=0.5)
+    x, args = logits.cuda().contiguous(), (actions.cuda(), old.cuda(), adv.cuda(), ref.cuda(), mask.cuda(), w.cuda())
+    got = ops.policy_loss(x, *args, ent_coef=0.01, kl_coef=0.1, scale=0.5)
+    tl, th, on = tol_logp(r, A), tol_entropy(r, A), r["on"].double()
+    # as for the loss above: what logp is off by, the roundings of old / ref - logp and of the products
+    step = tl + 8 * U + U * (clean.double().abs() + ref.double().abs() + r["logp"].abs())
+    dc = on * 0.5 * ww * (rho * adv.double().abs() + 0.1 * (torch.exp(d) + 1)) * step
+    lr = torch.log(rho)
+    tol = torch.stack([on * th, on * ((rho - 1).abs() * step + 16 * U * rho * lr.abs().clamp(min=0.01)), 0 * on, on * rho * step,
+                       on * ((torch.exp(d) - 1).abs() * step + 16 * U * (torch.exp(d) + 1) * d.abs().clamp(min=0.01)), 0 * on, dc + on * 0.5 * ww * 0.01 * th, on * U * ww])
+    check(got.stats, per_row.sum(1), tol.sum(1) + U * per_row.abs().sum(1), "stats")
+    for _ in range(2):
+        alone = ops.policy_loss(x, *args, ent_coef=0.01, kl_coef=0.1, scale=0.5, grad=False)
+        assert torch.equal(alone.stats, got.stats) and torch.equal(alone.logp, got.logp)
+
+
+@gpu
 @pytest.mark.parametrize("dt", list(DTYPES))
 @pytest.mark.parametrize("A", [6, 90, 700, 9001])
 def test_rows_with_nothing_to_learn(A, dt):

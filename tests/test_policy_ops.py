@@ -203,7 +203,7 @@ def test_against_64_bits(A, dt, masked):
 
 
 # the ends of the register sets a row may be held in (in 16-byte pieces): full, full with single values behind, and one piece more
-PIECES = [8, 16, 24, 32, 64, 96, 128, 192, 256, 384, 512, 768, 1024, 1536, 2048, 2560, 3072, 4096, 6144, 8192, 13312, 16384]
+PIECES = [8, 16, 24, 32, 64, 96, 128, 192, 256, 384, 512, 768, 1024, 1536, 2048, 2560, 3071, 3073, 4096, 6144, 8192, 13312, 16384]
 
 
 @gpu
@@ -213,7 +213,7 @@ PIECES = [8, 16, 24, 32, 64, 96, 128, 192, 256, 384, 512, 768, 1024, 1536, 2048,
 def test_ends_of_the_register_sets(pieces, dt, masked):
     dtype = DTYPES[dt]
     n = 4 if dt == "f32" else 8
-    for A in (pieces * n, pieces * n + n - 1, pieces * n + n):
+    for A in (pieces * n + 1, pieces * n + n - 1, pieces * n + n):
         rows = 131 if pieces > 4096 else 21               # (fewer rows of so many would be split)
         _, logits, actions, mask, g = make(rows, A, dtype, seed=6, masked=masked)
         x, act, m = logits.cuda(), actions.cuda(), None if mask is None else mask.cuda()

@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
             if (is_far(m)) { r.start(x0, k); sum(std::true_type{}); by = step_to(r.x0, r.m, x0, m, k); }
             else by = fmaxf(r.m - m, LOW);
             const float f = __builtin_amdgcn_exp2f(by);
-            float S = r.S(), Wt = f * fmaf(S, by, r.W());
-            S *= f;
+            // (scaled first: a lane that has nothing but a caller's -1e9 can hold an S of up to 2^127, whose product with `by` is not finite)
+            float S = f * r.S(), Wt = fmaf(S, by, f * r.W());
             if (G <= 64) { S = lanes<G, Sum>(S); Wt = lanes<G, Sum>(Wt); }
             else {
                 put_wave<G, Sum>(S, red[1]); put_wave<G, Sum>(Wt, red[2]);
@@ -449,7 +449,7 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(
     if (is_far(m)) { s.start(x0, g.k); sum(std::true_type{}); by = step_to(s.x0, s.m, x0, m, g.k); }
     else by = fmaxf(s.m - m, LOW);
     const float f = __builtin_amdgcn_exp2f(by);
-    put_wave<256, Sum>(f * s.S(), red[1]); put_wave<256, Sum>(f * fmaf(s.S(), by, s.W()), red[2]);
+    put_wave<256, Sum>(f * s.S(), red[1]); put_wave<256, Sum>(fmaf(f * s.S(), by, f * s.W()), red[2]);
     __syncthreads();
     const float S = get_waves<256, Sum>(red[1]), W = get_waves<256, Sum>(red[2]);
     if (lane == 0) { part[split] = x0; part[sp.splits + split] = S; part[2 * sp.splits + split] = W; }

@@ -1,0 +1,87 @@
+"""rlgymppo_cpp_amd.ops at the edges of what its calls accept: mask constants and temperatures of any size, logits next to the type's lowest value, infinities among
+a row's inputs, gradients of 40 decades, what autograd is told.  The definitions in 64 bits and the tolerances are those of test_policy_ops."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from rlgymppo_cpp_amd import _lib, ops
+from test_policy_ops import (DTYPES, FLOOR, U, check, check_clip, half_step, loss_inputs, make, ref_gradient, ref_loss, ref_rows, tol_entropy, tol_gradient,
+                             tol_logp)
+
+gpu = pytest.mark.gpu
+
+
+def check_row_calls(x, act, mask, temperature, g, some=None, size=1.0):
+    """All three calls on rows `some` of x against 64 bits; gradients of `size`; forbidden actions have exactly no gradient.  x, act, mask are on the CPU."""
+    rows, A = x.shape
+    dtype = x.dtype
+    some = torch.arange(rows) if some is None else some
+    xg, ag, mg = x.cuda(), act.cuda(), None if mask is None else mask.cuda()
+    sub = (x[some], act[some], None if mask is None else mask[some])
+    clean = sub[0] if mask is None else torch.where(sub[2], sub[0], torch.zeros_like(sub[0]))
+    r = ref_rows(clean, sub[1], sub[2], temperature)
+    zero = torch.zeros(len(some), dtype=torch.float64)
+    forbidden = torch.zeros_like(clean, dtype=torch.bool) if mask is None else ~sub[2]
+    logp, H = ops.action_logp(xg, ag, mg, temperature=temperature)
+    check(logp[some], r["logp"], tol_logp(r, A), "logp")
+    check(H[some], r["H"], tol_entropy(r, A), "entropy")
+    dl, dh = size * torch.randn(rows, generator=g), size * torch.randn(rows, generator=g)
+    c, h = torch.where(r["floored"] | ~r["on"], 0.0, dl[some].double()), torch.where(r["on"], dh[some].double(), 0.0)
+    want = ref_gradient(r, c, h, temperature)
+    for out in (None, xg.clone()):
+        got = ops.action_logp_backward(xg if out is None else out, ag, dl.cuda(), dh.cuda(), mg, temperature=temperature, out=out)[some]
+        check(got, want, tol_gradient(r, c, h, zero, want, dtype, temperature), f"dlogits (in place: {out is not None})")
+        assert (got[forbidden.cuda()] == 0).all()
+    old, adv, ref = loss_inputs(rows, g, torch.zeros(rows, dtype=torch.float64))
+    old[some] += r["logp"].float()
+    ref[some] += r["logp"].float()
+    rr, rho, d, ww, c, h, per_row = ref_loss(clean, sub[1], old[some], adv[some], ref[some], sub[2], None, ent=0.01, kl=0.1, temperature=temperature, scale=size)
+    want = ref_gradient(rr, c, h, temperature)
+    step = tol_logp(r, A) + 8 * U + U * (old[some].double().abs() + ref[some].double().abs() + r["logp"].abs())
+    dc = rr["on"].double() * size * (rho * adv[some].double().abs() + 0.1 * (torch.exp(d) + 1)) * step
+    for out in (None, xg.clone()):
+        res = ops.policy_loss(xg if out is None else out, ag, old.cuda(), adv.cuda(), ref.cuda(), mg, ent_coef=0.01, kl_coef=0.1, temperature=temperature, scale=size, out=out)
+        check(res.logp[some], r["logp"], tol_logp(r, A), "loss: logp")
+        check(res.dlogits[some], want, tol_gradient(rr, c, h, dc, want, dtype, temperature), f"loss: dlogits (in place: {out is not None})")
+        assert (res.dlogits[some][forbidden.cuda()] == 0).all()
+    if len(some) == rows:
+        th, on = tol_entropy(r, A), rr["on"].double()
+        check(res.stats[ops.STAT_ENTROPY], per_row[0].sum(), (on * th).sum() + U * per_row[0].abs().sum(), "loss: entropy")
+        check(res.stats[ops.STAT_LOSS], per_row[6].sum(), (dc + on * size * 0.01 * th).sum() + U * per_row[6].abs().sum(), "loss")
+        assert res.stats[ops.STAT_ROWS] == per_row[5].sum()
+
+
+# ---- masks by large negative logits ----------------------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("low,temperature", [(-1e9, 0.6), (-2e9, 1.2), (-4e9, 2.4), (-3e9, 1.0)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("A,rows,front", [(30, 9, 7), (90, 9, 22), (700, 9, 175), (700, 9, 20), (9000, 9, 2250), (9000, 9, 20), (40000, 9, 10000), (40000, 9, 20), (40000, 131, 20)])
+def test_masked_by_a_large_negative_logit(A, rows, front, dt, low, temperature):
+    """A lane that has nothing but the caller's -1e9: its exponents are past 2^30, where the rounding of one is itself an exponent of up to 2^7."""
+    _, x, act, _, g = make(rows, A, DTYPES[dt], seed=12, temperature=temperature)
+    x = x.clone()
+    x[:, front:] = low
+    act = (act % front).to(torch.int32)
+    check_row_calls(x, act, None, temperature, g, some=torch.arange(min(rows, 9)))
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_masked_by_a_large_negative_logit_of_any_size(dt):
+    """Mask constants over six decades and temperatures about 1: 20 logits in front of 70 of the constant."""
+    g = torch.Generator().manual_seed(3)
+    front = torch.randn((3, 20), generator=g)
+    for low in [-(10.0 ** (e / 7)) for e in range(49, 92)]:
+        for temperature in (0.45, 0.5, 0.6, 0.7, 0.77, 0.9, 1.0, 1.1, 1.2, 1.3, 1.7, 2.3):
+            x = torch.full((3, 90), low)
+            x[:, :20] = front
+            x = x.to(DTYPES[dt])
+            act = torch.tensor([0, 5, 19], dtype=torch.int32)
+            r = ref_rows(x, act, None, temperature)
+            logp, H = ops.action_logp(x.cuda(), act.cuda(), temperature=temperature)
+            check(logp, r["logp"], tol_logp(r, 90), f"logp, {low} at {temperature}")
+            check(H, r["H"], tol_entropy(r, 90), f"entropy, {low} at {temperature}")

@@ -157,7 +157,6 @@ __device__ __forceinline__ float step_to(float x0, float m, float new_x0, float 
 struct RowSum {
     float x0, m, s[2], w[2];
     __device__ __forceinline__ void clear() { x0 = LOWEST; m = -INFINITY; s[0] = s[1] = w[0] = w[1] = 0.f; }
-    __device__ __forceinline__ void start(float at, float k) { x0 = at; m = times_k(at, k); s[0] = s[1] = w[0] = w[1] = 0.f; }
     // `top`: the largest x of what comes next
     template <bool CAREFUL> __device__ __forceinline__ void reach(float top, float k) {
         const float to = times_k(top, k);
@@ -332,12 +331,22 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
             careful = !(fabsf(r.W()) < INFINITY);
             if (careful) { r.clear(); sum(std::true_type{}); }
             // the lanes' sums against the row's x0
-            if (G <= 64) x0 = lanes<G, Max>(r.x0);
-            else { put_wave<G, Max>(r.x0, red[0]); __syncthreads(); x0 = get_waves<G, Max>(red[0]); }
-            const float m = times_k(x0, k);
-            float by;
-            if (is_far(m)) { r.start(x0, k); sum(std::true_type{}); by = step_to(r.x0, r.m, x0, m, k); }
-            else by = fmaxf(r.m - m, LOW);
+            auto largest = [&]() {
+                if (G <= 64) return lanes<G, Max>(r.x0);
+                put_wave<G, Max>(r.x0, red[0]);
+                __syncthreads();
+                return get_waves<G, Max>(red[0]);
+            };
+            x0 = largest();
+            float m = times_k(x0, k), by;
+            if (is_far(m)) {
+                // (two of a far row's largest may be one exponent once rounded: the x0 of the quick sums need not be the larger)
+                r.clear();
+                sum(std::true_type{});
+                if (G > 64) __syncthreads();
+                x0 = largest(); m = times_k(x0, k);
+                by = step_to(r.x0, r.m, x0, m, k);
+            } else by = fmaxf(r.m - m, LOW);
             const float f = __builtin_amdgcn_exp2f(by);
             // (scaled first: a lane that has nothing but a caller's -1e9 can hold an S of up to 2^127, whose product with `by` is not finite)
             float S = f * r.S(), Wt = fmaf(S, by, f * r.W());
@@ -441,13 +450,15 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(
     s.clear();
     sum(std::false_type{});
     if (!(fabsf(s.W()) < INFINITY)) { s.clear(); sum(std::true_type{}); }
-    put_wave<256, Max>(s.x0, red[0]);
-    __syncthreads();
-    const float x0 = get_waves<256, Max>(red[0]);
-    const float m = times_k(x0, g.k);
-    float by;
-    if (is_far(m)) { s.start(x0, g.k); sum(std::true_type{}); by = step_to(s.x0, s.m, x0, m, g.k); }
-    else by = fmaxf(s.m - m, LOW);
+    auto largest = [&]() { put_wave<256, Max>(s.x0, red[0]); __syncthreads(); return get_waves<256, Max>(red[0]); };
+    float x0 = largest(), m = times_k(x0, g.k), by;
+    if (is_far(m)) {                                      // (as in k_rows)
+        s.clear();
+        sum(std::true_type{});
+        __syncthreads();
+        x0 = largest(); m = times_k(x0, g.k);
+        by = step_to(s.x0, s.m, x0, m, g.k);
+    } else by = fmaxf(s.m - m, LOW);
     const float f = __builtin_amdgcn_exp2f(by);
     put_wave<256, Sum>(f * s.S(), red[1]); put_wave<256, Sum>(fmaf(f * s.S(), by, f * s.W()), red[2]);
     __syncthreads();

@@ -85,3 +85,22 @@ def test_masked_by_a_large_negative_logit_of_any_size(dt):
             logp, H = ops.action_logp(x.cuda(), act.cuda(), temperature=temperature)
             check(logp, r["logp"], tol_logp(r, 90), f"logp, {low} at {temperature}")
             check(H, r["H"], tol_entropy(r, 90), f"entropy, {low} at {temperature}")
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1.0, 1e-3])
+@pytest.mark.parametrize("base", [1.5e9, 1.9e9, 3.9e9, -1.9e9, 7e9, 1.7e10, 1.3e20])
+@pytest.mark.parametrize("A,rows", [(90, 200), (700, 200), (9000, 150), (20000, 100), (20000, 130)])
+def test_largest_values_of_one_rounded_exponent(A, rows, base, temperature):
+    """Far rows whose largest logits are one or two of float32's steps apart, so that their rounded exponents may be one: the largest has all of the probability."""
+    g = torch.Generator().manual_seed(A + rows)
+    base = base * temperature
+    a = (base * (1 + 0.1 * torch.rand(rows, generator=g).double())).float()
+    x = a[:, None].expand(rows, A).clone()
+    x[:, ::7] -= abs(base) / 1000
+    inf = torch.full_like(a, math.inf)
+    act = torch.randint(0, A, (rows,), generator=g)
+    x[torch.arange(rows), act] = torch.nextafter(a, inf)
+    two = torch.arange(rows) % 2 == 0
+    x[torch.arange(rows)[two], act[two]] = torch.nextafter(torch.nextafter(a, inf), inf)[two]
+    check_row_calls(x, act.to(torch.int32), None, temperature, g, some=torch.randperm(rows, generator=g)[:64].sort().values if A > 5000 else None)

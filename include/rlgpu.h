@@ -395,8 +395,10 @@ typedef struct RlgpuPolicyRows {
 } RlgpuPolicyRows;
 /* Per row, over the allowed actions, with s = softmax(logits / temperature):
  *   logp = log max(s[action], min_prob)   (an action that is not allowed has s = 0),   entropy = -sum s log s   (0 log 0 = 0).
- * A row is LEFT OUT when its action is out of range or when nothing is allowed in it (mask all 0, or every allowed logit -inf or the type's lowest finite
- * value, or below -9e36): logp = entropy = 0 and its gradient is zero.  NaN and +inf among the allowed logits of a row give NaN.
+ * A logit of -1.875 * 2^122 (-9.97e36) or less, in float16 of -65504 (its lowest finite value) or less, counts as not allowed at any temperature, -inf among
+ * them: a mask written into the logits may use any of these.  Any other logit counts by the formula.
+ * A row is LEFT OUT when its action is out of range or when nothing is allowed in it: logp = entropy = 0 and its gradient is zero.  NaN and +inf among the
+ * allowed logits of a row give NaN.
  * entropy may be NULL.  Workspace: rlgpu_policy_workspace bytes (0: it may be NULL), 16-byte aligned, free again when the call's work on the stream is done. */
 int64_t rlgpu_policy_workspace(int32_t dtype, int32_t rows, int32_t n_actions, int32_t loss /* 1: for rlgpu_policy_loss, 0: for the other two */);   /* bytes; < 0: bad argument */
 int rlgpu_action_logp(int device, const RlgpuPolicyRows* p, float* logp, float* entropy, void* workspace, int64_t workspace_bytes, void* hip_stream);

@@ -11,7 +11,6 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
-#include <cstring>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -28,7 +27,7 @@ constexpr int64_t CACHE_BYTES = 256ll << 20, STREAM_BYTES = 2 * CACHE_BYTES;   /
 struct RowArgs {
     RlgpuPolicyRows p;
     float k, inv_t, log_floor;            // log2(e) / T, 1 / T, log(min_prob)
-    float none;                           // a row whose x0 is no larger has nothing allowed
+    float none, none_k;                   // Pack::LIMIT: a logit that is no larger is not allowed; its exponent, LIMIT k
     unsigned turn;
     float *logp, *entropy;                // optional
     const float *d_logp, *d_entropy;      // backward
@@ -85,11 +84,13 @@ using f32x2 = __attribute__((ext_vector_type(2))) float;
 using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 
-// N values of T in 16 bytes.  FILL, an action that is not allowed and places behind a row's end: low enough to be 0 in any sum, finite (an e t of 0 times -inf
-// would be NaN), and a row whose largest logit is no larger has nothing allowed (-9.97e36; float16: its lowest value, -65504).
+// N values of T in 16 bytes.  An action that is not allowed and places behind a row's end hold FILL (as a number LIMIT: -9.97e36; float16: its lowest value, -65504):
+// finite (an e t of 0 times -inf would be NaN), and 0 in any sum as long as its exponent is CLEAR of the row's.  Where it is not (a row's logits are next to it, or
+// the temperature makes it an ordinary exponent: float16 from T of about 590 on) CAREFUL sums leave it out by its value.  A caller's own logits of LIMIT or less
+// are so left out too: they are masks.
 template <typename T> struct Pack;
 template <> struct Pack<float> {
-    static constexpr int N = 4; static constexpr uint32_t FILL = 0xfcf00000u;
+    static constexpr int N = 4; static constexpr uint32_t FILL = 0xfcf00000u; static constexpr float LIMIT = -0x1.ep122f;
     static __device__ __forceinline__ float get(u32x4 v, int j) { const uint32_t w = v[j]; return __builtin_bit_cast(float, w); }   // (of v[j] itself the builtin takes element 0)
     static __device__ __forceinline__ u32x4 put(const float (&d)[4]) { u32x4 v; for (int j = 0; j < 4; j++) v[j] = __builtin_bit_cast(uint32_t, d[j]); return v; }
     using Bytes = uint32_t;                               // the mask of N values
@@ -117,12 +118,12 @@ template <typename T, typename T2> struct Pack16 {
     }
 };
 template <> struct Pack<__bf16> : Pack16<__bf16, bf16x2> {
-    static constexpr uint32_t FILL = 0xfcf0fcf0u;
+    static constexpr uint32_t FILL = 0xfcf0fcf0u; static constexpr float LIMIT = -0x1.ep122f;
     static __device__ __forceinline__ float get(u32x4 v, int j) { const uint32_t w = v[j >> 1]; return __builtin_bit_cast(float, j & 1 ? w & 0xffff0000u : w << 16); }
     static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xfcf0u); }
 };
 template <> struct Pack<_Float16> : Pack16<_Float16, f16x2> {
-    static constexpr uint32_t FILL = 0xfbfffbffu;
+    static constexpr uint32_t FILL = 0xfbfffbffu; static constexpr float LIMIT = -65504.f;
     static __device__ __forceinline__ float get(u32x4 v, int j) { return (float)__builtin_bit_cast(f16x2, (uint32_t)v[j >> 1])[j & 1]; }
     static __device__ __forceinline__ u32x4 forbid(u32x4 v, Bytes b) { return forbid16(v, b, 0xfbffu); }
 };
@@ -143,8 +144,9 @@ __device__ __forceinline__ void piece_done() { __builtin_amdgcn_sched_barrier(0)
 //
 // A quick sum can fail where logits are far from what a policy has: e t is NaN where t is -inf, and where k x passes FAR (the mask's FILL, a caller's -1e30) the
 // rounding of m would be an exponent itself.  W is then not finite, and the lane sums again with CAREFUL: against the exact maximum, with (x - x0) k for
-// k x - m where m is far, and no t below LOW.
+// k x - m where m is far, no t below LOW, and without what is not allowed.
 constexpr float SLACK = 8.f, FAR = 1e8f, LOWEST = -3.4028234663852886e38f;
+constexpr float CLEAR = 160.f;            // so far under m FILL's e is 0 (float32 ends at 2^-149)
 constexpr float LOW = -1e4f;              // 2^LOW is 0, and LOW times anything that occurs is finite: an exponent below is as good as LOW
 // k x0, rounded: left to itself the compiler joins the product with the difference that it is used in, and m would have another value in every place
 __device__ __forceinline__ float times_k(float x0, float k) {
@@ -153,6 +155,8 @@ __device__ __forceinline__ float times_k(float x0, float k) {
 }
 __device__ __forceinline__ bool is_far(float m) { return !(fabsf(m) < FAR); }
 __device__ __forceinline__ float exponent(float x, float k, float x0, float m) { return is_far(m) ? (x - x0) * k : fmaf(x, k, -m); }
+__device__ __forceinline__ float allowed(float x, float limit) { return x <= limit ? -INFINITY : x; }                 // (a NaN stays)
+__device__ __forceinline__ bool fill_shows(const RowArgs& g, float x0) { return !(fmaf(x0, g.k, -g.none_k) >= CLEAR); }   // (x0: within SLACK of the row's largest)
 __device__ __forceinline__ float step_to(float x0, float m, float new_x0, float new_m, float k) { return fmaxf(is_far(m) || is_far(new_m) ? (x0 - new_x0) * k : m - new_m, LOW); }
 struct RowSum {
     float x0, m, s[2], w[2];
@@ -166,7 +170,8 @@ struct RowSum {
             x0 = top; m = to;
         }
     }
-    template <bool CAREFUL> __device__ __forceinline__ void add(float x, float k, int j) {
+    template <bool CAREFUL, typename P> __device__ __forceinline__ void add(float x, float k, int j) {
+        if (CAREFUL) x = allowed(x, P::LIMIT);
         const float t = CAREFUL ? exponent(x, k, x0, m) : fmaf(x, k, -m), e = __builtin_amdgcn_exp2f(t);
         s[j] += e; w[j] = fmaf(e, CAREFUL ? fmaxf(t, LOW) : t, w[j]);
     }
@@ -176,7 +181,7 @@ struct RowSum {
         for (int j = 3; j + 1 < P::N; j += 2) top = max3(top, P::get(v, j), P::get(v, j + 1));
         reach<CAREFUL>(max3(top, P::get(v, P::N - 1), P::get(v, P::N - 1)), k);
 #pragma unroll
-        for (int j = 0; j < P::N; j++) add<CAREFUL>(P::get(v, j), k, j & 1);
+        for (int j = 0; j < P::N; j++) add<CAREFUL, P>(P::get(v, j), k, j & 1);
         asm("" : "+v"(v), "+v"(s[0]), "+v"(s[1]), "+v"(w[0]), "+v"(w[1]));
         piece_done();
     }
@@ -215,7 +220,7 @@ template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const Row
     if (!(x0 > g.none)) n.on = S != S;                    // nothing is allowed, but a NaN shows
     if (!n.on) return n;
     n.L = __builtin_amdgcn_logf(S);                       // (log2; S is about 1 at least)
-    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (exponent(xa, g.k, x0, times_k(x0, g.k)) - n.L);
+    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (exponent(allowed(xa, g.none), g.k, x0, times_k(x0, g.k)) - n.L);
     n.H = H < 0.f ? 0.f : H;                              // (the rounding of m can leave either an ulp of t off; a NaN stays)
     n.lpa = lpa > 0.f ? 0.f : (lpa < LOW ? LOW : lpa);    // (below every floor)
     const bool floored = n.lpa < g.log_floor;
@@ -227,14 +232,17 @@ template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const Row
 // The gradient of a piece: e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i).  The action's own c / T comes in a store of its own, of the lane that
 // wrote the 16 bytes around it.
 struct RowGradient {
-    float k, x0, m, p0, p1; bool careful;
-    __device__ __forceinline__ RowGradient(const RowArgs& g, const RowNumbers& n, float x0, bool careful) : k(g.k), x0(x0), m(times_k(x0, g.k)) {
+    float k, x0, m, p0, p1, limit; bool careful;
+    __device__ __forceinline__ RowGradient(const RowArgs& g, const RowNumbers& n, float x0, bool careful) : k(g.k), x0(x0), m(times_k(x0, g.k)), limit(g.none) {
         const float inv = g.inv_t * __builtin_amdgcn_exp2f(-n.L);
         p1 = -n.h * LN2 * inv; p0 = -(n.c + n.h * (n.H - LN2 * n.L)) * inv;
         this->careful = careful || is_far(m) || !(fabsf(p1) < 0.5f);   // an e_i of 0 times p1 t_i is 0 while that is finite: any t_i may be -3e38
     }
     __device__ __forceinline__ float quick(float x) const { const float t = fmaf(x, k, -m); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
-    __device__ __forceinline__ float of(float x) const { const float t = fmaxf(exponent(x, k, x0, m), LOW); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
+    __device__ __forceinline__ float of(float x) const {
+        const float t = fmaxf(exponent(x, k, x0, m), LOW);
+        return x <= limit ? 0.f : __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0);
+    }
     template <typename P> __device__ __forceinline__ u32x4 piece(u32x4 q) const {
         float d[P::N];
         if (careful) {
@@ -324,7 +332,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
                         for (int i = 0; i < BATCH; i++) r.template piece<CAREFUL, P>(q[i], k);
                     }
                 r.template reach<CAREFUL>(xt, k);
-                r.template add<CAREFUL>(xt, k, 1);
+                r.template add<CAREFUL, P>(xt, k, 1);
             };
             r.clear();
             sum(std::false_type{});
@@ -339,7 +347,9 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
             };
             x0 = largest();
             float m = times_k(x0, k), by;
-            if (is_far(m)) {
+            const bool shows = fill_shows(g, x0);
+            if (is_far(m) || shows) {
+                careful |= shows;
                 // (two of a far row's largest may be one exponent once rounded: the x0 of the quick sums need not be the larger)
                 r.clear();
                 sum(std::true_type{});
@@ -445,14 +455,14 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(
             for (int i = 0; i < 4; i++) s.template piece<CAREFUL, P>(q[i], g.k);
         }
         s.template reach<CAREFUL>(xt, g.k);
-        s.template add<CAREFUL>(xt, g.k, 1);
+        s.template add<CAREFUL, P>(xt, g.k, 1);
     };
     s.clear();
     sum(std::false_type{});
     if (!(fabsf(s.W()) < INFINITY)) { s.clear(); sum(std::true_type{}); }
     auto largest = [&]() { put_wave<256, Max>(s.x0, red[0]); __syncthreads(); return get_waves<256, Max>(red[0]); };
     float x0 = largest(), m = times_k(x0, g.k), by;
-    if (is_far(m)) {                                      // (as in k_rows)
+    if (is_far(m) || fill_shows(g, x0)) {                 // (as in k_rows)
         s.clear();
         sum(std::true_type{});
         __syncthreads();
@@ -789,9 +799,7 @@ template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM = false> 
 // Lanes and 16-byte pieces a row: the smallest set of registers that holds it.  Sums alone need no more of a row than what is in flight: 256 lanes take any.
 template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, int& blocks) {
     const int whole = g.p.n_actions / Pack<T>::N;
-    const uint32_t fill = Pack<T>::FILL; float low;
-    if (sizeof(T) == 2 && fill == 0xfbfffbffu) low = -65504.f; else { const uint32_t f = fill & 0xffff0000u; std::memcpy(&low, &f, 4); }
-    g.none = low;
+    g.none = Pack<T>::LIMIT; g.none_k = g.none * g.k;
     const int splits = splits_for(g.p.dtype, g.p.rows, g.p.n_actions);
     if (splits > 1) return launch_split<T, MODE>(g, s, splits, blocks);
     if (whole <= 8) return launch_rows_as<T, 8, 1, MODE, false>(g, s, blocks);

@@ -98,7 +98,8 @@ _stream = torch._C._cuda_getCurrentRawStream    # (device index) -> hipStream_t;
 
 def action_logp(logits, actions, mask=None, *, temperature=1.0, min_prob=MIN_PROB):
     """(logp, entropy) per row: log max(softmax(logits / temperature)[action], min_prob) and the softmax's entropy over the actions that `mask` (True =
-    allowed) lets through.  actions: int32; one outside [0, n_actions) leaves its row out, as a row in which nothing is allowed is: logp = entropy = 0."""
+    allowed) lets through; logits of -9.97e36 or less (float16: -65504) count as not allowed too.  actions: int32; one outside [0, n_actions) leaves its row
+    out, as a row in which nothing is allowed is: logp = entropy = 0."""
     p, rows, dev = _rows(logits, actions, mask, temperature, min_prob)
     lib = _lib.load()
     n = lib.rlgpu_policy_workspace(p.dtype, rows, p.n_actions, 0)

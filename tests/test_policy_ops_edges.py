@@ -21,10 +21,13 @@ def check_row_calls(x, act, mask, temperature, g, some=None, size=1.0):
     some = torch.arange(rows) if some is None else some
     xg, ag, mg = x.cuda(), act.cuda(), None if mask is None else mask.cuda()
     sub = (x[some], act[some], None if mask is None else mask[some])
-    clean = sub[0] if mask is None else torch.where(sub[2], sub[0], torch.zeros_like(sub[0]))
-    r = ref_rows(clean, sub[1], sub[2], temperature)
+    # logits that are masks by themselves
+    ok = ~(sub[0] <= (-65504.0 if dtype is torch.float16 else -1.875 * 2.0 ** 122))
+    ok = ok if mask is None else ok & sub[2]
+    clean = torch.where(ok, sub[0], torch.zeros_like(sub[0]))
+    r = ref_rows(clean, sub[1], ok, temperature)
     zero = torch.zeros(len(some), dtype=torch.float64)
-    forbidden = torch.zeros_like(clean, dtype=torch.bool) if mask is None else ~sub[2]
+    forbidden = ~ok
     logp, H = ops.action_logp(xg, ag, mg, temperature=temperature)
     check(logp[some], r["logp"], tol_logp(r, A), "logp")
     check(H[some], r["H"], tol_entropy(r, A), "entropy")
@@ -38,7 +41,7 @@ def check_row_calls(x, act, mask, temperature, g, some=None, size=1.0):
     old, adv, ref = loss_inputs(rows, g, torch.zeros(rows, dtype=torch.float64))
     old[some] += r["logp"].float()
     ref[some] += r["logp"].float()
-    rr, rho, d, ww, c, h, per_row = ref_loss(clean, sub[1], old[some], adv[some], ref[some], sub[2], None, ent=0.01, kl=0.1, temperature=temperature, scale=size)
+    rr, rho, d, ww, c, h, per_row = ref_loss(clean, sub[1], old[some], adv[some], ref[some], ok, None, ent=0.01, kl=0.1, temperature=temperature, scale=size)
     want = ref_gradient(rr, c, h, temperature)
     step = tol_logp(r, A) + 8 * U + U * (old[some].double().abs() + ref[some].double().abs() + r["logp"].abs())
     dc = rr["on"].double() * size * (rho * adv[some].double().abs() + 0.1 * (torch.exp(d) + 1)) * step
@@ -104,3 +107,80 @@ def test_largest_values_of_one_rounded_exponent(A, rows, base, temperature):
     two = torch.arange(rows) % 2 == 0
     x[torch.arange(rows)[two], act[two]] = torch.nextafter(torch.nextafter(a, inf), inf)[two]
     check_row_calls(x, act.to(torch.int32), None, temperature, g, some=torch.randperm(rows, generator=g)[:64].sort().values if A > 5000 else None)
+
+
+# ---- temperatures at which a type's lowest value is an ordinary exponent ------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("temperature", [500.0, 1e3, 2600.0, 1e4, 1e5])
+@pytest.mark.parametrize("A,rows", [(5, 9), (30, 9), (90, 67), (90, 1), (129, 9), (700, 9), (3001, 9), (9001, 9), (21001, 131), (50021, 1), (50021, 9), (50021, 131), (140001, 131)])
+def test_float16_at_high_temperatures(A, rows, temperature, masked):
+    """Forbidden actions and empty places have no probability, whatever 65504 / T is."""
+    _, x, act, mask, g = make(rows, A, torch.float16, seed=13, masked=masked, temperature=min(temperature, 3000.0))
+    if masked and rows > 4:
+        mask[4] = False
+    some = None if rows * A < 2_000_000 else torch.tensor([0, 1, 2, 4, rows - 1])
+    check_row_calls(x, act, mask, temperature, g, some=some, size=temperature)
+
+
+@gpu
+def test_a_forbidden_action_stays_at_the_floor():
+    """... also under a floor that is float32's smallest number."""
+    for dtype, temperature in [(torch.float16, t) for t in (1.0, 400.0, 700.0, 2600.0, 1e4, 1e6)] + [(torch.float32, 1e36), (torch.bfloat16, 1e36)]:
+        for A in (6, 90, 700, 40000):
+            x = torch.zeros((5, A), dtype=dtype, device="cuda")
+            mask = torch.ones((5, A), dtype=torch.bool, device="cuda")
+            mask[:, 1] = False
+            act = torch.ones(5, dtype=torch.int32, device="cuda")
+            for floor in (1e-11, 1e-45):
+                logp, H = ops.action_logp(x, act, mask, temperature=temperature, min_prob=floor)
+                assert (logp == np.float32(math.log(np.float32(floor)))).all(), (dtype, temperature, A)
+                assert (H.double() - math.log(A - 1)).abs().max() <= U * 2000 * math.log(A)
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1.0, 10.0, 100.0])
+@pytest.mark.parametrize("A,rows", [(30, 9), (90, 9), (1003, 9), (50021, 9), (50021, 131)])
+def test_float16_logits_next_to_the_lowest(A, rows, temperature):
+    """Rows whose largest logits are a few steps above -65504, some logits at it, in masked places too."""
+    g = torch.Generator().manual_seed(A)
+    x = (-65504.0 + 32.0 * torch.randint(0, 12, (rows, A), generator=g)).half()
+    act = torch.randint(0, A, (rows,), generator=g).to(torch.int32)
+    mask = torch.rand((rows, A), generator=g) < 0.7
+    mask[torch.arange(rows), act.long()] = True
+    x[2] = -65504.0                                         # left out
+    some = None if rows * A < 2_000_000 else torch.tensor([0, 1, 2, 4, rows - 1])
+    check_row_calls(x, act, mask, temperature, g, some=some)
+    check_row_calls(x, act, None, temperature, g, some=some)
+
+
+@gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("A,rows", [(30, 9), (90, 9), (1003, 9), (20011, 9), (50021, 9), (50021, 131)])
+def test_temperatures_near_the_largest_number(A, rows, dt, masked):
+    """Forbidden actions where float32's and bfloat16's numbers end as well."""
+    for temperature in (1e34, 1e35, 1e36):
+        _, x, act, mask, g = make(rows, A, DTYPES[dt], seed=14, masked=masked)
+        x = (x.float() * (temperature / 4)).to(DTYPES[dt])
+        some = None if rows * A < 2_000_000 else torch.tensor([0, 1, 2, 4, rows - 1])
+        check_row_calls(x, act, mask, temperature, g, some=some, size=1e30)
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("A", [90, 700, 40000])
+def test_where_a_row_begins_to_count(A, dt):
+    """A logit of -9.5e36 is one as any other; -1e37 is a mask (the limit is between them, -9.97e36)."""
+    x = torch.full((4, A), -1e37, dtype=DTYPES[dt], device="cuda")
+    x[0, 3] = -9.5e36
+    x[1] = -9.5e36
+    x[2, 3] = -math.inf
+    act = torch.full((4,), 3, dtype=torch.int32, device="cuda")
+    logp, H = ops.action_logp(x, act)
+    assert logp[0] == 0 and H[0] == 0
+    assert abs(float(logp[1]) + math.log(A)) < 1e-5 and abs(float(H[1]) - math.log(A)) < 1e-5
+    assert (logp[2:] == 0).all() and (H[2:] == 0).all()
+    d = ops.action_logp_backward(x, act, torch.ones(4, device="cuda"))
+    assert (d[2:] == 0).all() and float(d[1, 3]) > 0.9 and (d[0] == 0).all()

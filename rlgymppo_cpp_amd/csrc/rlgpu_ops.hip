@@ -222,9 +222,9 @@ template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const Row
     n.L = __builtin_amdgcn_logf(S);                       // (log2; S is about 1 at least)
     const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (exponent(allowed(xa, g.none), g.k, x0, times_k(x0, g.k)) - n.L);
     n.H = H < 0.f ? 0.f : H;                              // (the rounding of m can leave either an ulp of t off; a NaN stays)
-    n.lpa = lpa > 0.f ? 0.f : (lpa < LOW ? LOW : lpa);    // (below every floor)
+    n.lpa = xa <= g.none ? LOW : lpa > 0.f ? 0.f : (lpa < LOW ? LOW : lpa);    // (below every floor)
     const bool floored = n.lpa < g.log_floor;
-    n.logp = floored ? g.log_floor : n.lpa;
+    n.logp = lpa != lpa ? lpa : floored ? g.log_floor : n.lpa;
     if (MODE == BACKWARD) { n.c = floored ? 0.f : in.u; n.h = in.v; }
     if (MODE == LOSS) loss_row(g, in, n.logp, n.H, floored, n.c, n.h, st);
     return n;
@@ -236,7 +236,8 @@ struct RowGradient {
     __device__ __forceinline__ RowGradient(const RowArgs& g, const RowNumbers& n, float x0, bool careful) : k(g.k), x0(x0), m(times_k(x0, g.k)), limit(g.none) {
         const float inv = g.inv_t * __builtin_amdgcn_exp2f(-n.L);
         p1 = -n.h * LN2 * inv; p0 = -(n.c + n.h * (n.H - LN2 * n.L)) * inv;
-        this->careful = careful || is_far(m) || !(fabsf(p1) < 0.5f);   // an e_i of 0 times p1 t_i is 0 while that is finite: any t_i may be -3e38
+        // an e_i of 0 times p0 + p1 t_i is 0 while that is finite: any t_i may be -3e38
+        this->careful = careful || is_far(m) || !(fabsf(p1) < 0.5f && fabsf(p0) < INFINITY);
     }
     __device__ __forceinline__ float quick(float x) const { const float t = fmaf(x, k, -m); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
     __device__ __forceinline__ float of(float x) const {
@@ -254,7 +255,8 @@ struct RowGradient {
         }
         return P::put(d);
     }
-    static __device__ __forceinline__ float action(const RowArgs& g, const RowNumbers& n) { return (n.c - exp_of(n.lpa) * (n.c + n.h * (n.lpa + n.H))) * g.inv_t; }
+    // (a forbidden action has c = 0 and an lpa of LOW: no gradient, also where h is infinite)
+    static __device__ __forceinline__ float action(const RowArgs& g, const RowNumbers& n) { return n.lpa <= LOW ? 0.f : (n.c - exp_of(n.lpa) * (n.c + n.h * (n.lpa + n.H))) * g.inv_t; }
 };
 
 // G lanes take a row and hold it in registers, NV times 16 bytes each, from its one reading to the writing of the gradient.  What is over after the whole

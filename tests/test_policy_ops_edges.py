@@ -184,3 +184,36 @@ def test_where_a_row_begins_to_count(A, dt):
     assert (logp[2:] == 0).all() and (H[2:] == 0).all()
     d = ops.action_logp_backward(x, act, torch.ones(4, device="cuda"))
     assert (d[2:] == 0).all() and float(d[1, 3]) > 0.9 and (d[0] == 0).all()
+
+
+# ---- what is not finite ------------------------------------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("A", [6, 90, 700, 9001, 40001])
+def test_forbidden_actions_have_no_gradient_whatever_the_row_has(A, dt):
+    """Infinite and NaN gradients from above, and NaN and infinite logits among the allowed ones, do not reach the places that the mask forbids."""
+    dtype = DTYPES[dt]
+    g = torch.Generator().manual_seed(A)
+    R = 10
+    x = torch.randn((R, A), generator=g).to(dtype)
+    mask = torch.rand((R, A), generator=g) < 0.5
+    act = torch.full((R,), 1, dtype=torch.int32)
+    mask[:, 1] = True
+    mask[:, 2] = True
+    mask[:, 3] = False
+    act[7] = act[8] = 3                                     # forbidden actions
+    x[~mask] = math.nan
+    x[4, 2], x[5, 2], x[8, 2] = math.nan, math.inf, math.nan
+    dl = torch.tensor([math.inf, math.nan, 1.0, 1.0, 1.0, 1.0, -math.inf, 1.0, 3e38, 1.0])
+    dh = torch.tensor([1.0, 0.0, math.inf, math.nan, 1.0, 1.0, 1.0, math.inf, 1.0, 3e38])
+    xg, ag, mg = x.cuda(), act.cuda(), mask.cuda()
+    for temperature in (1.0, 0.01, 3e3):
+        d = ops.action_logp_backward(xg, ag, dl.cuda(), dh.cuda(), mg, temperature=temperature)
+        assert (d[~mg] == 0).all()
+        assert d[4][mg[4]].isnan().all() and d[5][mg[5]].isnan().all()
+        if temperature >= 1.0:                              # (at 0.01 logits 0.25 apart are 25 apart in log-probability: the action may be at the floor, which passes none)
+            assert not d[0, 1].isfinite() and d[1, 1].isnan()
+        adv = torch.tensor([math.inf, math.nan, 1.0, 1.0, 1.0, 1.0, -math.inf, 1.0, 3e38, 1.0]).cuda()
+        r = ops.policy_loss(xg, ag, torch.full((R,), -1.0).cuda(), adv, None, mg, ent_coef=0.5, scale=1e3, temperature=temperature)
+        assert (r.dlogits[~mg] == 0).all() and r.dlogits[4][mg[4]].isnan().all()

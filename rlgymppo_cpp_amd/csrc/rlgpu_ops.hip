@@ -45,6 +45,8 @@ __device__ __forceinline__ float exp_minus_1_minus(float x) {
     const float near = x * x * (0.5f + x * (1.f / 6 + x * (1.f / 24 + x * (1.f / 120 + x * (1.f / 720 + x * (1.f / 5040 + x * (1.f / 40320)))))));
     return fabsf(x) < 0.25f ? near : exp_of(x) - 1.f - x;
 }
+// exp(x) - 1, from that sum only where it is small against x: behind a reference that rules an action out, x is far below 0 or -inf
+__device__ __forceinline__ float exp_minus_1(float x, float minus_x) { return fabsf(x) < 0.25f ? minus_x + x : exp_of(x) - 1.f; }
 
 // what a row's numbers need besides its logits, asked for before the sums over them
 struct RowInputs { float w, u, v, ref; };                 // weight; d_logp and d_entropy, or old_logp and adv; ref_logp
@@ -66,7 +68,7 @@ __device__ __forceinline__ void loss_row(const RowArgs& g, const RowInputs& in, 
     if (l.ref_logp) {
         const float d = in.ref - logp;
         ref = exp_minus_1_minus(d);
-        if (l.kl_coef != 0.f) { value += l.kl_coef * ref; c -= l.kl_coef * (ref + d); }      // (ref + d: exp(d) - 1)
+        if (l.kl_coef != 0.f) { value += l.kl_coef * ref; c -= l.kl_coef * exp_minus_1(d, ref); }
     }
     value -= l.ent_coef * H;
     c = floored ? 0.f : c * w * l.scale;

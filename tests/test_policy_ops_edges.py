@@ -217,3 +217,29 @@ def test_forbidden_actions_have_no_gradient_whatever_the_row_has(A, dt):
         adv = torch.tensor([math.inf, math.nan, 1.0, 1.0, 1.0, 1.0, -math.inf, 1.0, 3e38, 1.0]).cuda()
         r = ops.policy_loss(xg, ag, torch.full((R,), -1.0).cuda(), adv, None, mg, ent_coef=0.5, scale=1e3, temperature=temperature)
         assert (r.dlogits[~mg] == 0).all() and r.dlogits[4][mg[4]].isnan().all()
+
+
+@gpu
+def test_a_reference_that_rules_the_action_out():
+    """ref_logp far below logp, down to -inf (an action that the reference's own mask forbids): the KL term's derivative is 1 - exp(d), to float32's last bits."""
+    refs = [-math.inf, -1e30, -1e8, -1e6, -1e4, -1000.0, -300.0, -90.0, -50.0, -20.0, -5.0, -2.5, -1.7, -1.2]
+    R, A = len(refs), 6
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn((R, A), generator=g)
+    act = torch.arange(R).remainder(A).to(torch.int32)
+    r = ref_rows(x, act)
+    old = r["logp"].float()
+    ref, adv = torch.tensor(refs), torch.zeros(R)
+    got = ops.policy_loss(x.cuda(), act.cuda(), old.cuda(), adv.cuda(), ref.cuda(), kl_coef=0.5)
+    d = ref.double() - r["logp"]
+    c = -0.5 * torch.expm1(d)
+    want = ref_gradient(r, c, 0 * c, 1.0)
+    # d is off by what logp is off and its own rounding, exp(d) by that and by its own 4 u; nothing of it grows with |d| beyond exp(d) |d|
+    step = tol_logp(r, A) + U * d.abs().clamp(max=200)
+    dc = 0.5 * (torch.exp(d) * (step + 4 * U) + 2 * U)
+    check(got.dlogits, want, tol_gradient(r, c, 0 * c, dc, want, torch.float32, 1.0), "dlogits")
+    assert got.stats[ops.STAT_LOSS] == math.inf and got.stats[ops.STAT_REF_KL] == math.inf
+    less = ops.policy_loss(x[5:].cuda(), act[5:].cuda(), old[5:].cuda(), adv[5:].cuda(), ref[5:].cuda(), kl_coef=0.5)
+    want = 0.5 * (torch.expm1(d) - d)[5:].sum()
+    tol = 0.5 * (torch.expm1(d).abs() * step + 16 * U * (torch.exp(d) + 1 + d.abs()))
+    assert abs(float(less.stats[ops.STAT_LOSS]) - want) <= float(tol[5:].sum())

@@ -61,7 +61,8 @@ __device__ __forceinline__ void loss_row(const RowArgs& g, const RowInputs& in, 
     const RlgpuPolicyLoss& l = g.loss;
     const float x = logp - in.u, adv = in.v, w = in.w;
     const float r = exp_of(x);
-    const float surr = r * adv, clipped = fminf(fmaxf(r, 1.f - l.clip_low), 1.f + l.clip_high) * adv;
+    const float surr = adv == 0.f && r == INFINITY ? 0.f : r * adv;       // (a ratio past float32's range)
+    const float clipped = fminf(fmaxf(r, 1.f - l.clip_low), 1.f + l.clip_high) * adv;
     float value = -(clipped < surr ? clipped : surr);     // (a NaN in either stays: surr holds it)
     c = clipped < surr ? 0.f : -surr;
     float ref = 0.f;

@@ -243,3 +243,16 @@ def test_a_reference_that_rules_the_action_out():
     want = 0.5 * (torch.expm1(d) - d)[5:].sum()
     tol = 0.5 * (torch.expm1(d).abs() * step + 16 * U * (torch.exp(d) + 1 + d.abs()))
     assert abs(float(less.stats[ops.STAT_LOSS]) - want) <= float(tol[5:].sum())
+
+
+@gpu
+def test_an_advantage_of_zero_has_no_loss():
+    """... also where the ratio is past float32's range."""
+    x = torch.zeros((3, 5), device="cuda")
+    act = torch.zeros(3, dtype=torch.int32, device="cuda")
+    old = torch.tensor([-95.0, -200.0, -1.0], device="cuda")
+    r = ops.policy_loss(x, act, old, torch.zeros(3, device="cuda"))
+    assert r.stats[ops.STAT_LOSS] == 0 and (r.dlogits == 0).all()
+    assert r.stats[ops.STAT_CLIPPED] == 3 and r.stats[ops.STAT_RATIO] == math.inf
+    r = ops.policy_loss(x, act, old, torch.tensor([2.0, 0.0, 0.0], device="cuda"))
+    assert abs(float(r.stats[ops.STAT_LOSS]) + 2.4) < 1e-6 and (r.dlogits == 0).all()

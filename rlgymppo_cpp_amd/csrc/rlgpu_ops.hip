@@ -272,13 +272,14 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
     using P = Pack<T>;
     constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = MODE == LOGP ? 4 : 2;
     constexpr bool AHEAD = G == 1024;
-    __shared__ float red[3][W], sums[RPB][STATS];
+    __shared__ float red[3][W];
+    __shared__ double sums[RPB][STATS];                   // the loss's statistics: a workgroup may have 2^19 rows
     const int lane = G <= 64 ? threadIdx.x % G : threadIdx.x, sub = G <= 64 ? threadIdx.x / G : 0;
     const int A = g.p.n_actions, whole = A / N, rest = A - whole * N, groups = (g.p.rows + RPB - 1) / RPB;
     const float k = g.k;
     const bool masked = g.p.mask != nullptr;
     u32x4 v[NV];
-    if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] = 0.f;   // (kept by the row's first lane)
+    if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] = 0;     // (kept by the row's first lane)
     auto row_at = [&](int pass) { return (pass * (int)gridDim.x + (int)((blockIdx.x + (unsigned)pass * g.turn) % gridDim.x)) * RPB + sub; };
     auto logits = [&](int row) { return (const T*)g.p.logits + row_offset(row, g.p.ld); };
     int row = row_at(0), a = -1; float w = 0.f;
@@ -374,7 +375,8 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
             float st[STATS];
             n = row_numbers<MODE>(g, in, x0, S, Wt, xa, st);
             on = n.on;
-            if (MODE == LOSS && on && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] += st[j];
+            // (added in LDS: one instruction, and none of the sums in a register; nobody else adds to them)
+            if (MODE == LOSS && on && lane == 0) for (int j = 0; j < STATS; j++) __hip_atomic_fetch_add(&sums[sub][j], (double)st[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
         const bool ahead = AHEAD && counts(next_a, next_w);
         const T* next_x = logits(ahead ? next : 0);
@@ -416,9 +418,9 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
     if (MODE != LOSS) return;
     __syncthreads();
     if (threadIdx.x < STATS) {
-        float s = sums[0][threadIdx.x];
+        double s = sums[0][threadIdx.x];
         for (int j = 1; j < RPB; j++) s += sums[j][threadIdx.x];
-        g.row_stats[(int64_t)blockIdx.x * STATS + threadIdx.x] = s;
+        g.row_stats[(int64_t)blockIdx.x * STATS + threadIdx.x] = (float)s;
     }
 }
 

@@ -256,3 +256,20 @@ def test_an_advantage_of_zero_has_no_loss():
     assert r.stats[ops.STAT_CLIPPED] == 3 and r.stats[ops.STAT_RATIO] == math.inf
     r = ops.policy_loss(x, act, old, torch.tensor([2.0, 0.0, 0.0], device="cuda"))
     assert abs(float(r.stats[ops.STAT_LOSS]) + 2.4) < 1e-6 and (r.dlogits == 0).all()
+
+
+# ---- sums ----------------------------------------------------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("R,A", [((1 << 26) + 77, 2), (3_000_001, 90)])
+def test_statistics_of_millions_of_rows(R, A):
+    """Rows that are all the same: what is added up has the rounding of a workgroup's sum and of the total, not one for every row."""
+    x = torch.zeros((R, A), device="cuda")
+    x[:, 0] = 0.7
+    act = torch.zeros(R, dtype=torch.int32, device="cuda")
+    old, adv = torch.full((R,), -0.31, device="cuda"), torch.full((R,), 0.37, device="cuda")
+    ref, w = torch.full((R,), -0.9, device="cuda"), torch.full((R,), 1.1, device="cuda")
+    kw = dict(ent_coef=0.01, kl_coef=0.1, scale=0.3, grad=False)
+    one = ops.policy_loss(x[:1], act[:1], old[:1], adv[:1], ref[:1], None, w[:1], **kw).stats.double()
+    got = ops.policy_loss(x, act, old, adv, ref, None, w, **kw).stats.double()
+    assert ((got - R * one).abs() <= 2 * U * R * one.abs()).all(), got / (R * one) - 1

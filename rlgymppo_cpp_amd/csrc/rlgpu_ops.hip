@@ -681,8 +681,9 @@ template <typename B> __global__ void __launch_bounds__(256) k_grad_scale(B b, c
     const double norm = (double)grad_scale * sqrt(s);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const double scale = (double)grad_scale * fmin(1.0, (double)max_norm / (norm + 1e-6));
-    // in two factors: gradients near float32's largest value are scaled by less than its smallest normal one (f0 is a power of two, and 1 elsewhere)
-    const float f0 = scale < 0x1p-100 ? 0x1p-64f : 1.f, f = (float)(scale < 0x1p-100 ? scale * 0x1p64 : scale);
+    // in two factors: gradients near float32's largest value are scaled by less than its smallest normal one.  f0 is a power of two, 1 elsewhere, and small enough
+    // for f to be a normal number wherever a product can be one (scale >= 2^-252), with g f0 still normal there
+    const float f0 = scale < 0x1p-180 ? 0x1p-126f : scale < 0x1p-100 ? 0x1p-64f : 1.f, f = (float)(scale / (double)f0);
     // not a norm to clip by (as the caller sees it, in 32 bits), or nothing to clip
     if (!((float)norm < INFINITY) || (grad_scale == 1.f && norm + 1e-6 <= (double)max_norm)) return;
     for_pieces(b, true, [&](int, int t, int64_t at, int n) {

@@ -273,3 +273,21 @@ def test_statistics_of_millions_of_rows(R, A):
     one = ops.policy_loss(x[:1], act[:1], old[:1], adv[:1], ref[:1], None, w[:1], **kw).stats.double()
     got = ops.policy_loss(x, act, old, adv, ref, None, w, **kw).stats.double()
     assert ((got - R * one).abs() <= 2 * U * R * one.abs()).all(), got / (R * one) - 1
+
+
+@gpu
+def test_clip_by_a_factor_under_float32_s_smallest():
+    """Gradients near float32's largest value, clipped to norms of 10^-18 and less: the factor is under 2^-190, the result an ordinary number."""
+    for norm in (1e-18, 1e-20, 1e-25, 1e-30, 1e-36):
+        g = torch.Generator().manual_seed(1)
+        a = (torch.randn(300, generator=g) * 1e37).cuda()
+        b = (torch.randn(77, generator=g) * 1e37).bfloat16().cuda()
+        before = [a.clone(), b.clone()]
+        got = ops.clip_grad_norm([a, b], norm)
+        exact = math.sqrt(sum(float((t.double() ** 2).sum()) for t in before))
+        assert abs(float(got) - exact) <= 2 * U * exact
+        for t, was in zip((a, b), before):
+            want = was.double().cpu() * (norm / (exact + 1e-6))
+            check(t, want, (half_step(t.dtype) + 4 * U) * want.abs() + 2.0 ** (-133 if t.dtype is torch.bfloat16 else -148), f"clipped to {norm}")
+    for scale in (2.0 ** -126, 2.0 ** -140):
+        check_clip([(torch.randn(300) * 1e30).cuda()], math.inf, scale)

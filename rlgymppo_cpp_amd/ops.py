@@ -8,7 +8,8 @@ PPOLearner: PPO/DiscretePolicy.cpp:44-75, PPO/PPOLearner.cpp:148-215, 273-288).
 
 Tensors live on one GPU; the work goes to that device's current torch stream, and the outputs are new tensors of it.  Nothing synchronises and nothing is
 kept between calls, so a call may be captured into a graph.  The gradients are explicit calls, not autograd nodes: no call looks at requires_grad.
-Arguments that do not fit raise ValueError before anything runs; an error of the library raises RlgpuError.
+What is written in place (out=, clipped gradients) counts as modified for autograd, as after torch's own in-place operations: a graph that kept it for its
+backward pass raises there.  Arguments that do not fit raise ValueError before anything runs; an error of the library raises RlgpuError.
 """
 import ctypes as C
 from array import array
@@ -93,6 +94,7 @@ def _gradient(out, logits):
     return out
 
 
+_written = torch.autograd.graph.increment_version    # of a tensor or several: the kernels write behind autograd's back
 _stream = torch._C._cuda_getCurrentRawStream    # (device index) -> hipStream_t; torch.cuda.current_stream(device).cuda_stream without the object around it: 2 us less a call
 
 
@@ -115,19 +117,21 @@ def action_logp(logits, actions, mask=None, *, temperature=1.0, min_prob=MIN_PRO
 
 def action_logp_backward(logits, actions, d_logp, d_entropy=None, mask=None, *, temperature=1.0, min_prob=MIN_PROB, out=None):
     """The gradient of sum(d_logp * logp + d_entropy * entropy) with respect to the logits, in the logits' type.  A logp at the floor passes none, rows left
-    out and actions that are not allowed get 0.  out: where to write it; `logits` itself may be given."""
+    out and actions that are not allowed get 0.  out: where to write it; `logits` itself may be given, unless the layer behind it keeps its output (a tanh, a softmax)."""
     p, rows, dev = _rows(logits, actions, mask, temperature, min_prob)
     c = _vector("d_logp", d_logp, rows, torch.float32, dev)
     h = _vector("d_entropy", d_entropy, rows, torch.float32, dev) if d_entropy is not None else None
-    out = _gradient(out, logits)
-    ld = _row_stride("out", out, rows, logits.shape[1])
+    d = _gradient(out, logits)
+    ld = _row_stride("out", d, rows, logits.shape[1])
     lib = _lib.load()
     n = lib.rlgpu_policy_workspace(p.dtype, rows, p.n_actions, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    rc = lib.rlgpu_action_logp_backward(dev.index, C.byref(p), c, h, out.data_ptr(), ld, ws.data_ptr() if n else None, n, _stream(dev.index))
+    rc = lib.rlgpu_action_logp_backward(dev.index, C.byref(p), c, h, d.data_ptr(), ld, ws.data_ptr() if n else None, n, _stream(dev.index))
     if rc:
         _fail(rc)
-    return out
+    if out is not None:
+        _written(out)
+    return d
 
 
 def policy_loss(logits, actions, old_logp, adv, ref_logp=None, mask=None, weights=None, *, clip_range=0.2, clip_high=None, ent_coef=0.0, kl_coef=0.0,
@@ -161,6 +165,8 @@ def policy_loss(logits, actions, old_logp, adv, ref_logp=None, mask=None, weight
     rc = lib.rlgpu_policy_loss(dev.index, C.byref(p), C.byref(l), ws_at, n, _stream(dev.index))
     if rc:
         _fail(rc)
+    if out is not None:
+        _written(out)
     return PolicyLoss(stats, logp, dlogits)
 
 
@@ -203,6 +209,8 @@ def clip_grad_norm(grads, max_norm=float("inf"), grad_scale=1.0):
                                   ws.data_ptr(), size, _stream(dev.index))
     if rc:
         _fail(rc)
+    if max_norm < float("inf") or grad_scale != 1.0:
+        _written(grads)
     return norm
 
 

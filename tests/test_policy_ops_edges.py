@@ -291,3 +291,36 @@ def test_clip_by_a_factor_under_float32_s_smallest():
             check(t, want, (half_step(t.dtype) + 4 * U) * want.abs() + 2.0 ** (-133 if t.dtype is torch.bfloat16 else -148), f"clipped to {norm}")
     for scale in (2.0 ** -126, 2.0 ** -140):
         check_clip([(torch.randn(300) * 1e30).cuda()], math.inf, scale)
+
+
+# ---- autograd ------------------------------------------------------------------------------------------------------------------------------------------------
+
+@gpu
+def test_autograd_hears_of_what_is_written():
+    """A layer that keeps its output for its own gradient (a soft cap) raises when the gradient was written over it, as after torch's own in-place operations."""
+    x = torch.randn((9, 90), device="cuda", requires_grad=True)
+    act = torch.zeros(9, dtype=torch.int32, device="cuda")
+    v = torch.ones(9, device="cuda")
+    for call in (lambda y: ops.action_logp_backward(y, act, v, out=y), lambda y: ops.policy_loss(y, act, -v, v, out=y).dlogits,
+                 lambda y: ops.action_logp_backward(y.detach().clone(), act, v, out=y.detach())):
+        y = torch.tanh(x)
+        d = call(y)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward(d.detach())
+        y = 5.0 * torch.tanh(x / 5.0)                       # (a product keeps its inputs, not its output)
+        y.backward(call(y).detach())
+    # a gradient that another graph keeps
+    p = torch.ones(5, device="cuda", requires_grad=True)
+    grad = torch.full((5,), 2.0, device="cuda")
+    z = (p * grad).sum()
+    before = grad._version
+    ops.clip_grad_norm([grad])                              # the norm alone writes nothing
+    assert grad._version == before
+    ops.clip_grad_norm([grad, torch.ones(3, device="cuda")], 0.5)
+    assert grad._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    with torch.inference_mode():
+        q = torch.ones((2, 4), device="cuda")
+        ops.action_logp_backward(q, act[:2], v[:2], out=q)
+        ops.clip_grad_norm([q], 0.5)

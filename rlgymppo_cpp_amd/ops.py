@@ -91,10 +91,13 @@ def _gradient(out, logits):
         raise ValueError("out: a tensor of the logits' shape, type and device is needed")
     if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ValueError("out: its rows overlap")
+    if out.requires_grad and out.is_leaf and torch.is_grad_enabled():
+        raise ValueError("out: a leaf that requires a gradient (write over it under torch.no_grad())")
     return out
 
 
 _written = torch.autograd.graph.increment_version    # of a tensor or several: the kernels write behind autograd's back
+_PLAIN = {torch.Tensor}
 _stream = torch._C._cuda_getCurrentRawStream    # (device index) -> hipStream_t; torch.cuda.current_stream(device).cuda_stream without the object around it: 2 us less a call
 
 
@@ -174,7 +177,8 @@ def clip_grad_norm(grads, max_norm=float("inf"), grad_scale=1.0):
     """grad_scale * sqrt(sum of the squares of all the tensors' values) as a float32 tensor of one value; the tensors are multiplied in place by
     grad_scale * min(1, max_norm / (norm + 1e-6)), as PPOCore.clip_adam_step does.  max_norm = inf with grad_scale = 1 only takes the norm.  A norm that is
     not finite leaves the tensors as they are: look at it before the step.  grads: dense tensors (contiguous, or a permutation of it) of one GPU in float32,
-    bfloat16 or float16, in any mix; None entries (parameters without a gradient) are passed over.  Tensors that overlap are refused when they are written."""
+    bfloat16 or float16, in any mix; None entries (parameters without a gradient) are passed over.  Tensors that overlap, and parameters in the place of their
+    gradients, are refused when they are written."""
     grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
     if not grads:
         raise ValueError("grads: no tensor")
@@ -182,6 +186,9 @@ def clip_grad_norm(grads, max_norm=float("inf"), grad_scale=1.0):
         raise ValueError(f"max_norm: {max_norm}")
     if not 0.0 < grad_scale < float("inf"):
         raise ValueError(f"grad_scale: {grad_scale}")
+    writes = max_norm < float("inf") or grad_scale != 1.0
+    if writes and not _PLAIN.issuperset(map(type, grads)) and any(isinstance(g, torch.nn.Parameter) for g in grads):
+        raise ValueError("grads: a parameter is among them (the gradients are its .grad)")
     # a pass over the list for each thing asked, with nothing but the tensor's own method in it: a network has hundreds of tensors, and a GPU that waits
     try:
         ptrs, counts = array("Q", map(torch.Tensor.data_ptr, grads)), array("q", map(torch.Tensor.numel, grads))
@@ -209,7 +216,7 @@ def clip_grad_norm(grads, max_norm=float("inf"), grad_scale=1.0):
                                   ws.data_ptr(), size, _stream(dev.index))
     if rc:
         _fail(rc)
-    if max_norm < float("inf") or grad_scale != 1.0:
+    if writes:
         _written(grads)
     return norm
 

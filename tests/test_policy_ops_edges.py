@@ -324,3 +324,29 @@ def test_autograd_hears_of_what_is_written():
         q = torch.ones((2, 4), device="cuda")
         ops.action_logp_backward(q, act[:2], v[:2], out=q)
         ops.clip_grad_norm([q], 0.5)
+
+
+def test_what_may_not_be_written():
+    """Parameters in the place of gradients, and leaves that require a gradient, are refused before anything runs."""
+    net = torch.nn.Linear(3, 2)
+    with pytest.raises(ValueError, match="parameter"):
+        ops.clip_grad_norm(net.parameters(), 0.5)
+    with pytest.raises(ValueError, match="parameter"):
+        ops.clip_grad_norm([torch.zeros(3), net.bias], 0.5)
+    with pytest.raises(ValueError, match="parameter"):
+        ops.clip_grad_norm(net.weight, math.inf, 0.5)
+    with pytest.raises(ValueError, match="GPU"):            # their norm may be taken
+        ops.clip_grad_norm(net.parameters())
+
+
+@gpu
+def test_a_leaf_may_not_be_written():
+    x = torch.zeros((2, 6), device="cuda", requires_grad=True)
+    a, v = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.ones(2, device="cuda")
+    with pytest.raises(ValueError, match="leaf"):
+        ops.action_logp_backward(x, a, v, out=x)
+    with pytest.raises(ValueError, match="leaf"):
+        ops.policy_loss(x, a, v, v, out=x)
+    with torch.no_grad():
+        ops.action_logp_backward(x, a, v, out=x)
+    assert float(x.detach()[0, 0]) > 0.8

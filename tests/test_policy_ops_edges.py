@@ -350,3 +350,25 @@ def test_a_leaf_may_not_be_written():
     with torch.no_grad():
         ops.action_logp_backward(x, a, v, out=x)
     assert float(x.detach()[0, 0]) > 0.8
+
+
+@gpu
+def test_outputs_are_tensors_of_their_own():
+    """What happens to one output does not count as a change of another."""
+    x = torch.randn((9, 90), device="cuda")
+    act = torch.zeros(9, dtype=torch.int32, device="cuda")
+    v = torch.ones(9, device="cuda")
+    p = torch.ones(9, device="cuda", requires_grad=True)
+    logp, H = ops.action_logp(x, act)
+    y = (p * H).sum()
+    logp += 1.0
+    y.backward()
+    assert torch.equal(p.grad, H)
+    r = ops.policy_loss(x, act, logp, v)
+    p.grad = None
+    y = (p * r.logp).sum()
+    r.stats.zero_()
+    y.backward()
+    assert torch.equal(p.grad, r.logp)
+    for t in (logp, H, r.logp, r.stats):
+        assert t.untyped_storage().nbytes() == t.numel() * 4

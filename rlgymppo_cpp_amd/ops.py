@@ -108,10 +108,12 @@ def action_logp(logits, actions, mask=None, *, temperature=1.0, min_prob=MIN_PRO
     p, rows, dev = _rows(logits, actions, mask, temperature, min_prob)
     lib = _lib.load()
     n = lib.rlgpu_policy_workspace(p.dtype, rows, p.n_actions, 0)
-    # (outputs of one allocation would be one tensor to autograd: what is done to one counts as a change of the other)
-    logp, entropy = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    rc = lib.rlgpu_action_logp(dev.index, C.byref(p), logp.data_ptr(), entropy.data_ptr(), ws.data_ptr() if n else None, n, _stream(dev.index))
+    # one allocation: the workspace in front (none for most sizes), then the outputs
+    buf = torch.empty(n // 4 + 2 * rows, dtype=torch.float32, device=dev)
+    _, logp, entropy = buf.split_with_sizes((n // 4, rows, rows))
+    entropy = entropy.data                              # (its own version counter: what is done to logp is no change of it)
+    at = buf.data_ptr()
+    rc = lib.rlgpu_action_logp(dev.index, C.byref(p), at + n, at + n + 4 * rows, at, n, _stream(dev.index))
     if rc:
         _fail(rc)
     return logp, entropy
@@ -159,10 +161,13 @@ def policy_loss(logits, actions, old_logp, adv, ref_logp=None, mask=None, weight
         raise ValueError("out: without a gradient there is nothing to write")
     lib = _lib.load()
     n = lib.rlgpu_policy_workspace(p.dtype, rows, p.n_actions, 1)
-    stats, logp = torch.empty(8, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    l = _lib.PolicyLossC(old_at, adv_at, ref_at, weights_at, clip_range, clip_high, ent_coef, kl_coef, scale, logp.data_ptr(), stats.data_ptr(), to, ld)
-    rc = lib.rlgpu_policy_loss(dev.index, C.byref(p), C.byref(l), ws.data_ptr(), n, _stream(dev.index))
+    # one allocation: the workspace in front, then the statistics and the log-probabilities
+    buf = torch.empty(n // 4 + 8 + rows, dtype=torch.float32, device=dev)
+    _, stats, logp = buf.split_with_sizes((n // 4, 8, rows))
+    stats = stats.data                                  # (its own version counter)
+    ws_at = buf.data_ptr()
+    l = _lib.PolicyLossC(old_at, adv_at, ref_at, weights_at, clip_range, clip_high, ent_coef, kl_coef, scale, ws_at + n + 32, ws_at + n, to, ld)
+    rc = lib.rlgpu_policy_loss(dev.index, C.byref(p), C.byref(l), ws_at, n, _stream(dev.index))
     if rc:
         _fail(rc)
     if out is not None:

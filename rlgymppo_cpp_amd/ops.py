@@ -37,8 +37,11 @@ def _fail(rc):
 
 
 def _vector(name, t, rows, dtype, dev):
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 1 and t.numel() == rows and t.is_contiguous() and t.device == dev:
-        return t.data_ptr()
+    try:
+        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 1 and t.numel() == rows and t.is_contiguous() and t.device == dev:
+            return t.data_ptr()
+    except RuntimeError:                                    # a sparse tensor has neither strides nor memory of its own
+        raise ValueError(f"{name}: a strided tensor is needed") from None
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != 1 or t.numel() != rows:
         raise ValueError(f"{name}: a {str(dtype)[6:]} tensor of {rows} rows is needed")
     if t.device != dev:
@@ -47,7 +50,10 @@ def _vector(name, t, rows, dtype, dev):
 
 
 def _row_stride(name, t, rows, n):
-    ld, one = t.stride()
+    try:
+        ld, one = t.stride()
+    except RuntimeError:
+        raise ValueError(f"{name}: a strided tensor is needed") from None
     if n > 1 and one != 1:
         raise ValueError(f"{name}: the actions of a row have to be adjacent")
     return ld if rows > 1 else n
@@ -87,8 +93,8 @@ def _rows(logits, actions, mask, temperature, min_prob):
 def _gradient(out, logits):
     if out is None:
         return torch.empty_like(logits, memory_format=torch.contiguous_format)
-    if not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.dtype is not logits.dtype or out.device != logits.device:
-        raise ValueError("out: a tensor of the logits' shape, type and device is needed")
+    if not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.dtype is not logits.dtype or out.device != logits.device or out.layout is not torch.strided:
+        raise ValueError("out: a strided tensor of the logits' shape, type and device is needed")
     if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ValueError("out: its rows overlap")
     if out.requires_grad and out.is_leaf and torch.is_grad_enabled():
@@ -198,6 +204,8 @@ def clip_grad_norm(grads, max_norm=float("inf"), grad_scale=1.0):
         devices = set(map(torch.Tensor.get_device, grads))
     except TypeError:
         raise ValueError("grads: tensors (or None) are needed") from None
+    except RuntimeError:
+        raise ValueError("grads: strided tensors are needed (a sparse one is among them)") from None
     try:
         kinds = array("i", [_DTYPES[g.dtype] for g in grads])
     except KeyError as e:

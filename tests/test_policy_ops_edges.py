@@ -370,3 +370,20 @@ def test_outputs_are_tensors_of_their_own():
     r.stats.zero_()
     y.backward()
     assert torch.equal(p.grad, r.logp)
+
+
+# ---- refusals ------------------------------------------------------------------------------------------------------------------------------------------------
+
+def test_sparse_tensors_are_refused():
+    s = torch.eye(4).to_sparse()
+    x, a, v = torch.zeros((4, 4)), torch.zeros(4, dtype=torch.int32), torch.zeros(4)
+    with pytest.raises(ValueError, match="strided"):
+        ops.clip_grad_norm([torch.zeros(3), s], 1.0)
+    with pytest.raises(ValueError, match="logits"):
+        ops.action_logp(s, a)
+    with pytest.raises(ValueError, match="mask"):
+        ops.action_logp(x, a, s.bool())
+    with pytest.raises(ValueError, match="actions"):
+        ops.action_logp(x, a.to_sparse())
+    with pytest.raises(ValueError, match="adv"):
+        ops.policy_loss(x, a, v, v.to_sparse())

@@ -376,7 +376,7 @@ def test_outputs_are_tensors_of_their_own():
 
 def test_sparse_tensors_are_refused():
     s = torch.eye(4).to_sparse()
-    x, a, v = torch.zeros((4, 4)), torch.zeros(4, dtype=torch.int32), torch.zeros(4)
+    x, a = torch.zeros((4, 4)), torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ValueError, match="strided"):
         ops.clip_grad_norm([torch.zeros(3), s], 1.0)
     with pytest.raises(ValueError, match="logits"):
@@ -385,5 +385,14 @@ def test_sparse_tensors_are_refused():
         ops.action_logp(x, a, s.bool())
     with pytest.raises(ValueError, match="actions"):
         ops.action_logp(x, a.to_sparse())
+
+
+@gpu
+def test_sparse_row_vectors_and_outputs_are_refused():
+    x, a, v = torch.zeros((4, 4), device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(4, device="cuda")
     with pytest.raises(ValueError, match="adv"):
         ops.policy_loss(x, a, v, v.to_sparse())
+    with pytest.raises(ValueError, match="weights"):
+        ops.policy_loss(x, a, v, v, weights=v.to_sparse())
+    with pytest.raises(ValueError, match="out"):
+        ops.action_logp_backward(x, a, v, out=x.to_sparse())

@@ -387,11 +387,11 @@ const char* rlgpu_lt_last_error(void);
  * an error: rlgpu_ops_last_error() (of the calling thread). */
 enum { RLGPU_F32 = 0, RLGPU_BF16 = 1, RLGPU_F16 = 2 };
 typedef struct RlgpuPolicyRows {
-    const void* logits; int64_t ld;           /* [rows][n_actions], row stride `ld` in elements (n_actions .. 2^31), any alignment of a row */
+    const void* logits; int64_t ld;           /* [rows][n_actions], row stride `ld` in elements (n_actions .. 2^31 - 1), any alignment of a row */
     const uint8_t* mask; int64_t ld_mask;     /* optional [rows][n_actions]: 0 = the action is not allowed, its logit is not looked at (it may be NaN); ld_mask 0: one row for all */
     const int32_t* actions;                   /* [rows]; an index outside 0 .. n_actions - 1 leaves the row out */
     int32_t dtype, rows, n_actions;           /* RLGPU_F32 / BF16 / F16, 0 <= rows <= 2^30, 1 <= n_actions <= 2^28 */
-    float temperature, min_prob;              /* > 0; the floor of a probability, 0 < min_prob < 1 (rlgpu_policy_act: 1e-11) */
+    float temperature, min_prob;              /* > 0, log2(e) / temperature finite in float32 (from 4.24e-39 on); the floor of a probability, 0 < min_prob < 1 (rlgpu_policy_act: 1e-11) */
 } RlgpuPolicyRows;
 /* Per row, over the allowed actions, with s = softmax(logits / temperature):
  *   logp = log max(s[action], min_prob)   (an action that is not allowed has s = 0),   entropy = -sum s log s   (0 log 0 = 0).

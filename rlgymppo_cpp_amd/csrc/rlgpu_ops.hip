@@ -720,6 +720,7 @@ struct OnDevice {
 int64_t size_of(int dtype) { return dtype == RLGPU_F32 ? 4 : (dtype == RLGPU_BF16 || dtype == RLGPU_F16 ? 2 : 0); }
 bool misaligned(const void* p, int64_t to) { return (uintptr_t)p % (uintptr_t)to != 0; }
 
+float exponents(float temperature) { return (float)(1.4426950408889634 / (double)temperature); }     // k
 int64_t policy_bytes(int dtype, int rows, int n_actions, bool loss);
 
 int check_rows(const char* who, const RlgpuPolicyRows* p, const void* workspace, int64_t bytes, bool loss = false) {
@@ -727,7 +728,7 @@ int check_rows(const char* who, const RlgpuPolicyRows* p, const void* workspace,
     const int64_t size = size_of(p->dtype);
     if (!size) return fail(RLGPU_ERR_ARG, "%s: dtype %d is none of RLGPU_F32, RLGPU_BF16, RLGPU_F16", who, p->dtype);
     if (p->rows < 0 || p->rows > (1 << 30) || p->n_actions < 1 || p->n_actions > (1 << 28)) return fail(RLGPU_ERR_ARG, "%s: %d rows of %d actions", who, p->rows, p->n_actions);
-    if (!(p->temperature > 0.f) || !(p->temperature < INFINITY) || !(1.f / p->temperature < INFINITY)) return fail(RLGPU_ERR_ARG, "%s: temperature %g", who, (double)p->temperature);
+    if (!(p->temperature > 0.f) || !(p->temperature < INFINITY) || !(exponents(p->temperature) < INFINITY)) return fail(RLGPU_ERR_ARG, "%s: temperature %g", who, (double)p->temperature);
     if (!(p->min_prob > 0.f && p->min_prob < 1.f)) return fail(RLGPU_ERR_ARG, "%s: min_prob %g is not between 0 and 1", who, (double)p->min_prob);
     if (p->rows == 0) return RLGPU_OK;
     if (!p->logits || !p->actions) return fail(RLGPU_ERR_ARG, "%s: logits and actions are needed", who);
@@ -756,7 +757,7 @@ int check_gradient(const char* who, const RlgpuPolicyRows* p, const void* dlogit
 RowArgs row_args(const RlgpuPolicyRows* p) {
     RowArgs g{};
     g.p = *p;
-    g.inv_t = 1.f / p->temperature; g.k = (float)(1.4426950408889634 / (double)p->temperature); g.log_floor = (float)std::log((double)p->min_prob);
+    g.inv_t = 1.f / p->temperature; g.k = exponents(p->temperature); g.log_floor = (float)std::log((double)p->min_prob);
     return g;
 }
 // workgroups of a kernel that the device keeps at once (a second, partly filled round would leave most of it idle)

@@ -374,6 +374,17 @@ def test_outputs_are_tensors_of_their_own():
 
 # ---- refusals ------------------------------------------------------------------------------------------------------------------------------------------------
 
+def test_a_temperature_whose_reciprocal_is_no_float():
+    """log2(e) / T has to be a float32 as well as 1 / T."""
+    lib = _lib.load()
+    P = 1 << 20
+    for temperature in (2.95e-39, 3.5e-39, 4.2e-39, 1e-39):
+        p = _lib.PolicyRows(logits=P, ld=6, mask=None, ld_mask=0, actions=P, dtype=0, rows=4, n_actions=6, temperature=temperature, min_prob=1e-11)
+        # (logp is null: refused all the same, if later)
+        assert lib.rlgpu_action_logp(0, C.byref(p), None, None, P, 1 << 20, None) == -1
+        assert b"temperature" in lib.rlgpu_ops_last_error(), temperature
+
+
 def test_sparse_tensors_are_refused():
     s = torch.eye(4).to_sparse()
     x, a = torch.zeros((4, 4)), torch.zeros(4, dtype=torch.int32)

@@ -27,7 +27,7 @@ constexpr int64_t CACHE_BYTES = 256ll << 20, STREAM_BYTES = 2 * CACHE_BYTES;   /
 struct RowArgs {
     RlgpuPolicyRows p;
     float k, inv_t, log_floor;            // log2(e) / T, 1 / T, log(min_prob)
-    float none, none_k;                   // Pack::LIMIT: a logit that is no larger is not allowed; its exponent, LIMIT k
+    float none, near;                     // Pack::LIMIT: a logit that is no larger is not allowed; the least m that is neither far nor within CLEAR of LIMIT k
     unsigned turn;
     float *logp, *entropy;                // optional
     const float *d_logp, *d_entropy;      // backward
@@ -159,7 +159,7 @@ __device__ __forceinline__ float times_k(float x0, float k) {
 __device__ __forceinline__ bool is_far(float m) { return !(fabsf(m) < FAR); }
 __device__ __forceinline__ float exponent(float x, float k, float x0, float m) { return is_far(m) ? (x - x0) * k : fmaf(x, k, -m); }
 __device__ __forceinline__ float allowed(float x, float limit) { return x <= limit ? -INFINITY : x; }                 // (a NaN stays)
-__device__ __forceinline__ bool fill_shows(const RowArgs& g, float x0) { return !(fmaf(x0, g.k, -g.none_k) >= CLEAR); }   // (x0: within SLACK of the row's largest)
+__device__ __forceinline__ bool needs_care(const RowArgs& g, float m) { return !(m >= g.near && m < FAR); }   // far, or FILL shows
 __device__ __forceinline__ float step_to(float x0, float m, float new_x0, float new_m, float k) { return fmaxf(is_far(m) || is_far(new_m) ? (x0 - new_x0) * k : m - new_m, LOW); }
 struct RowSum {
     float x0, m, s[2], w[2];
@@ -223,11 +223,11 @@ template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const Row
     if (!(x0 > g.none)) n.on = S != S;                    // nothing is allowed, but a NaN shows
     if (!n.on) return n;
     n.L = __builtin_amdgcn_logf(S);                       // (log2; S is about 1 at least)
-    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (exponent(allowed(xa, g.none), g.k, x0, times_k(x0, g.k)) - n.L);
+    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (exponent(xa, g.k, x0, times_k(x0, g.k)) - n.L);
     n.H = H < 0.f ? 0.f : H;                              // (the rounding of m can leave either an ulp of t off; a NaN stays)
     n.lpa = xa <= g.none ? LOW : lpa > 0.f ? 0.f : (lpa < LOW ? LOW : lpa);    // (below every floor)
     const bool floored = n.lpa < g.log_floor;
-    n.logp = lpa != lpa ? lpa : floored ? g.log_floor : n.lpa;
+    n.logp = floored ? g.log_floor : n.lpa;
     if (MODE == BACKWARD) { n.c = floored ? 0.f : in.u; n.h = in.v; }
     if (MODE == LOSS) loss_row(g, in, n.logp, n.H, floored, n.c, n.h, st);
     return n;
@@ -240,7 +240,7 @@ struct RowGradient {
         const float inv = g.inv_t * __builtin_amdgcn_exp2f(-n.L);
         p1 = -n.h * LN2 * inv; p0 = -(n.c + n.h * (n.H - LN2 * n.L)) * inv;
         // an e_i of 0 times p0 + p1 t_i is 0 while that is finite: any t_i may be -3e38
-        this->careful = careful || is_far(m) || !(fabsf(p1) < 0.5f && fabsf(p0) < INFINITY);
+        this->careful = careful || !(fmaf(fabsf(p0), 0x1p-126f, fabsf(p1)) < 0.5f);
     }
     __device__ __forceinline__ float quick(float x) const { const float t = fmaf(x, k, -m); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
     __device__ __forceinline__ float of(float x) const {
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
     const float k = g.k;
     const bool masked = g.p.mask != nullptr;
     u32x4 v[NV];
-    if (MODE == LOSS && lane == 0) for (int j = 0; j < STATS; j++) sums[sub][j] = 0;     // (kept by the row's first lane)
+    if (MODE == LOSS && lane < STATS) sums[sub][lane] = 0;
     auto row_at = [&](int pass) { return (pass * (int)gridDim.x + (int)((blockIdx.x + (unsigned)pass * g.turn) % gridDim.x)) * RPB + sub; };
     auto logits = [&](int row) { return (const T*)g.p.logits + row_offset(row, g.p.ld); };
     int row = row_at(0), a = -1; float w = 0.f;
@@ -353,9 +353,8 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
             };
             x0 = largest();
             float m = times_k(x0, k), by;
-            const bool shows = fill_shows(g, x0);
-            if (is_far(m) || shows) {
-                careful |= shows;
+            if (needs_care(g, m)) {
+                careful = true;
                 // (two of a far row's largest may be one exponent once rounded: the x0 of the quick sums need not be the larger)
                 r.clear();
                 sum(std::true_type{});
@@ -375,8 +374,12 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
             float st[STATS];
             n = row_numbers<MODE>(g, in, x0, S, Wt, xa, st);
             on = n.on;
-            // (added in LDS: one instruction, and none of the sums in a register; nobody else adds to them)
-            if (MODE == LOSS && on && lane == 0) for (int j = 0; j < STATS; j++) __hip_atomic_fetch_add(&sums[sub][j], (double)st[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            // (a lane for each statistic; added in LDS, so that no sum is in a register: nobody else adds to it)
+            if (MODE == LOSS && on && lane < STATS) {
+                const float a0 = lane & 1 ? st[1] : st[0], a1 = lane & 1 ? st[3] : st[2], a2 = lane & 1 ? st[5] : st[4], a3 = lane & 1 ? st[7] : st[6];
+                const float b0 = lane & 2 ? a1 : a0, b1 = lane & 2 ? a3 : a2;
+                __hip_atomic_fetch_add(&sums[sub][lane], (double)(lane & 4 ? b1 : b0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
         }
         const bool ahead = AHEAD && counts(next_a, next_w);
         const T* next_x = logits(ahead ? next : 0);
@@ -469,7 +472,7 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(
     if (!(fabsf(s.W()) < INFINITY)) { s.clear(); sum(std::true_type{}); }
     auto largest = [&]() { put_wave<256, Max>(s.x0, red[0]); __syncthreads(); return get_waves<256, Max>(red[0]); };
     float x0 = largest(), m = times_k(x0, g.k), by;
-    if (is_far(m) || fill_shows(g, x0)) {                 // (as in k_rows)
+    if (needs_care(g, m)) {                 // (as in k_rows)
         s.clear();
         sum(std::true_type{});
         __syncthreads();
@@ -808,7 +811,7 @@ template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM = false> 
 // Lanes and 16-byte pieces a row: the smallest set of registers that holds it.  Sums alone need no more of a row than what is in flight: 256 lanes take any.
 template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, int& blocks) {
     const int whole = g.p.n_actions / Pack<T>::N;
-    g.none = Pack<T>::LIMIT; g.none_k = g.none * g.k;
+    g.none = Pack<T>::LIMIT; g.near = std::max(g.none * g.k + CLEAR, -FAR);
     const int splits = splits_for(g.p.dtype, g.p.rows, g.p.n_actions);
     if (splits > 1) return launch_split<T, MODE>(g, s, splits, blocks);
     if (whole <= 8) return launch_rows_as<T, 8, 1, MODE, false>(g, s, blocks);

@@ -267,8 +267,12 @@ struct RowGradient {
 // batches, and for the gradient once more.  Workgroups stay for row after row; the rows of a pass over the grid are turned by `turn`, so that sequences padded at
 // the same places do not leave some workgroups all the padding.  With 1024 lanes only one workgroup fits a CU, and it asks for its next row's pieces as it
 // writes the last's gradient: otherwise memory would wait for the sums and the sums for memory.
+//
+// Wavefronts a SIMD are asked for where they pay: 8 for the gradient of short rows (in 16 bits 2 to 8 registers spill for it: 1.5 M rows of 90 float16 actions 166 us
+// against 190 without, 1 M of 128 116 and 128, but 335 544 of 400 124 and 119), 6 for the loss of up to 3 pieces a lane (one register fewer: 191 739 rows of 700
+// bfloat16 actions 124 and 128 us).
 template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM>
-__global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACKWARD && G <= 16 ? 8 : 1) k_rows(RowArgs g) {
+__global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACKWARD && G <= 16 ? 8 : MODE == LOSS && G <= 64 && NV <= 3 ? 6 : 1) k_rows(RowArgs g) {
     using P = Pack<T>;
     constexpr int N = P::N, RPB = G <= 64 ? 256 / G : 1, W = G <= 64 ? 1 : G / 64, BATCH = MODE == LOGP ? 4 : 2;
     constexpr bool AHEAD = G == 1024;
@@ -429,7 +433,8 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
 
 // ---- few rows of many actions: a row over `splits` workgroups, `per` pieces each ---------------------------------------------------------------------------
 // k_parts leaves x0, S and W of its part in part[row][split] and the action's logit behind the row's parts (the gradient may overwrite it before another part of
-// the row is done); k_join adds a row's parts up in every workgroup that needs them, in the same order, and writes the outputs and its part of the gradient.
+// the row is done); k_join adds a row's parts up in every workgroup that needs them and writes the outputs and its part of the gradient.  (Those workgroups join in
+// the same order; the one of the loss's statistics has fewer lanes for a row and another order, and its last bits may not be those of logp and the gradient.)
 struct SplitArgs { int splits, per; float* part; };      // part: [rows][3 * splits + 1]
 template <typename T, Mode MODE> __device__ __forceinline__ bool row_counts(const RowArgs& g, int row, int& a, float& w) {
     a = g.p.actions[row]; w = MODE == LOSS && g.loss.weights ? g.loss.weights[row] : 1.f;
@@ -763,13 +768,15 @@ RowArgs row_args(const RlgpuPolicyRows* p) {
     g.inv_t = 1.f / p->temperature; g.k = exponents(p->temperature); g.log_floor = (float)std::log((double)p->min_prob);
     return g;
 }
-// workgroups of a kernel that the device keeps at once (a second, partly filled round would leave most of it idle)
-template <typename K> int resident(K kernel, int threads) {
+// Workgroups of a kernel that the device keeps at once (a second, partly filled round would leave most of it idle).  `waves`: of a SIMD as its 800 scalar registers
+// have room for them, which the query does not count: 8 with up to 80 each, 7 with up to 96, 6 with the 112 that most of the kernels have that write a gradient
+// (loss of 33 554 rows of 4 000 float32 actions on a grid for 7 wavefronts, where 6 fit: 249 us, on one for 6: 215).
+template <typename K> int resident(K kernel, int threads, int waves) {
     int device = 0, cus = 256, per_cu = 1;
     (void)hipGetDevice(&device);
     (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess) { (void)hipGetLastError(); per_cu = 1; }
-    return std::max(1, std::min(ROW_BLOCKS, cus * per_cu));
+    return std::max(1, std::min(ROW_BLOCKS, cus * std::min(per_cu, waves * 4 * 64 / threads)));
 }
 // Few rows of many actions: a workgroup a row would leave the device idle.  Parts of at least a piece a lane, as many as give every CU two.  Measured in parts
 // and as a workgroup a row, us for the backward pass in bfloat16: 131 072 actions 6.6 and 17.1 for 1 row, 8.9 and 18.2 for 32, 20.0 and 21.9 for 128, 34.4 and
@@ -797,7 +804,9 @@ template <typename T, Mode MODE> int launch_split(RowArgs& g, hipStream_t s, int
 }
 template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM = false> int launch_rows_as(RowArgs& g, hipStream_t s, int& blocks) {
     constexpr int threads = G <= 64 ? 256 : G, rpb = threads / G;
-    static const int most = resident(&k_rows<T, G, NV, MODE, MORE, STREAM>, threads);
+    // (512 lanes of a loss: two workgroups a CU and not three, 201 and 212 us for 12 201 rows of 11 000 float32 actions)
+    constexpr int waves = MODE == LOGP || (MODE == BACKWARD && G <= 16) ? 8 : MODE == BACKWARD && G <= 64 ? 7 : MODE == LOSS && G == 512 ? 4 : 6;
+    static const int most = resident(&k_rows<T, G, NV, MODE, MORE, STREAM>, threads, waves);
     const int groups = (g.p.rows + rpb - 1) / rpb, passes = (groups + most - 1) / most;
     blocks = (groups + passes - 1) / passes;              // as many rows for each (2 048 groups: 1 024 workgroups twice, 12.1 us, not 1 536 and then 512, 12.5)
     g.turn = blocks * 5u / 13u;

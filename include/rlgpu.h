@@ -423,7 +423,8 @@ typedef struct RlgpuPolicyLoss {
 } RlgpuPolicyLoss;
 #define RLGPU_POLICY_STATS 8
 int rlgpu_policy_loss(int device, const RlgpuPolicyRows* p, const RlgpuPolicyLoss* loss, void* workspace, int64_t workspace_bytes, void* hip_stream);
-/* clip_grad_norm over n_tensors dense tensors (host arrays of device pointers, element counts and RLGPU_* types; counts may be 0; up to 2^40 elements each):
+/* clip_grad_norm over n_tensors dense tensors (host arrays of device pointers, element counts and RLGPU_* types; counts may be 0; up to 2^24
+ * tensors of up to 2^40 elements each):
  *   *norm = grad_scale * sqrt(sum over all tensors of g^2)  (device, fp32; summed in 64 bits in a fixed order),
  *   g *= grad_scale * min(1, max_norm / (*norm + 1e-6))  in place, as rlgpu_clip_adam_step clips.
  * A norm that is not finite leaves every gradient as it is.  max_norm = +inf with grad_scale = 1 only takes the norm and writes no gradient; any other call

@@ -56,7 +56,8 @@ template <Mode MODE> __device__ __forceinline__ RowInputs row_inputs(const RowAr
     if (MODE == LOSS) { r.u = g.loss.old_logp[row]; r.v = g.loss.adv[row]; if (g.loss.ref_logp) r.ref = g.loss.ref_logp[row]; }
     return r;
 }
-// one row of the loss: d loss / d logp and d loss / d entropy, and the row's part of the statistics
+// one row of the loss: d loss / d logp and d loss / d entropy, and the row's part of the statistics.  In 32 bits, as logp itself is, whose error of a few 2^-24 is
+// the larger one: a ratio that is nearer than that to a border of the clip can fall on either side of it, and counts there in the statistics too.
 __device__ __forceinline__ void loss_row(const RowArgs& g, const RowInputs& in, float logp, float H, bool floored, float& c, float& h, float (&st)[STATS]) {
     const RlgpuPolicyLoss& l = g.loss;
     const float x = logp - in.u, adv = in.v, w = in.w;
@@ -139,7 +140,8 @@ template <bool STREAM> __device__ __forceinline__ void store(void* p, u32x4 v) {
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c)); return r; }
 
 // Between two pieces of a row.  Left alone, the scheduler unpacks every piece first and adds later, as the sums are one long chain, or keeps the 32-bit values of
-// one pass for the next (219 registers where 32 hold a row in 16 bits, and spills in the largest).
+// one pass for the next (219 registers where 32 hold a row in 16 bits).  The sets of 16 pieces a lane are at the limit of 128 registers all the same: their gradient
+// spills 4 to 6 in 16 bits, the loss 8 to 10 in float32 and 20 to 23 in 16 bits, once a row.
 __device__ __forceinline__ void piece_done() { __builtin_amdgcn_sched_barrier(0); }
 
 // What a lane has of S and W.  `m` is the exponent (k x0) that its sums are taken against: not the maximum, but within SLACK of it, so that it hardly ever moves
@@ -862,6 +864,7 @@ int64_t policy_bytes(int dtype, int rows, int n_actions, bool loss) {
     return splits > 1 ? (int64_t)rows * (3 * splits + 1) * 4 : (loss ? stats_bytes(rows) : 0);
 }
 
+constexpr int MOST_TENSORS = 1 << 24;     // (their partial sums are counted in 32 bits)
 int clip_batches(int n) { return std::max(1, (n + TENSORS - 1) / TENSORS); }
 int clip_share(int n_batches) { return std::max(256, 2 * CLIP_BLOCKS / n_batches); }   // workgroups of a launch, so that the partial sums stay few
 
@@ -969,14 +972,14 @@ int rlgpu_policy_loss(int device, const RlgpuPolicyRows* p, const RlgpuPolicyLos
 }
 
 int64_t rlgpu_clip_grad_workspace(int32_t n) {
-    if (n < 0) return fail(RLGPU_ERR_ARG, "rlgpu_clip_grad_workspace: %d tensors", n);
+    if (n < 0 || n > MOST_TENSORS) return fail(RLGPU_ERR_ARG, "rlgpu_clip_grad_workspace: %d tensors", n);
     return (int64_t)clip_batches(n) * clip_share(clip_batches(n)) * 8;
 }
 
 int rlgpu_clip_grad_norm(int device, int32_t n, void* const* grads, const int64_t* counts, const int32_t* dtypes, float max_norm, float grad_scale,
                          float* norm, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* who = "rlgpu_clip_grad_norm";
-    if (n < 0 || (n && (!grads || !counts || !dtypes))) return fail(RLGPU_ERR_ARG, "%s: %d tensors", who, n);
+    if (n < 0 || n > MOST_TENSORS || (n && (!grads || !counts || !dtypes))) return fail(RLGPU_ERR_ARG, "%s: %d tensors", who, n);
     if (!(max_norm >= 0.f)) return fail(RLGPU_ERR_ARG, "%s: max_norm %g", who, (double)max_norm);
     if (!(grad_scale > 0.f && grad_scale < INFINITY)) return fail(RLGPU_ERR_ARG, "%s: grad_scale %g", who, (double)grad_scale);
     if (!norm || misaligned(norm, 4)) return fail(RLGPU_ERR_ARG, "%s: norm is needed", who);

@@ -385,6 +385,16 @@ def test_a_temperature_whose_reciprocal_is_no_float():
         assert b"temperature" in lib.rlgpu_ops_last_error(), temperature
 
 
+def test_more_tensors_than_can_be_counted():
+    lib = _lib.load()
+    P = 1 << 20
+    for n in ((1 << 24) + 1, (1 << 31) - 1, (1 << 31) - 100):
+        assert lib.rlgpu_clip_grad_workspace(n) < 0
+        # (no array is looked at)
+        assert lib.rlgpu_clip_grad_norm(0, n, P, P, P, 1.0, 1.0, P, P, 1 << 40, None) == -1 and b"tensors" in lib.rlgpu_ops_last_error()
+    assert lib.rlgpu_clip_grad_workspace(1 << 24) > 0
+
+
 def test_sparse_tensors_are_refused():
     s = torch.eye(4).to_sparse()
     x, a = torch.zeros((4, 4)), torch.zeros(4, dtype=torch.int32)

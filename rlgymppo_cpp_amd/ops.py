@@ -7,9 +7,10 @@ PPOLearner: PPO/DiscretePolicy.cpp:44-75, PPO/PPOLearner.cpp:148-215, 273-288).
     norm = ops.clip_grad_norm([p.grad for p in network.parameters()], 0.5)
 
 Tensors live on one GPU; the work goes to that device's current torch stream, and the outputs are new tensors of it.  Nothing synchronises and nothing is
-kept between calls, so a call may be captured into a graph.  The gradients are explicit calls, not autograd nodes: no call looks at requires_grad.
-What is written in place (out=, clipped gradients) counts as modified for autograd, as after torch's own in-place operations: a graph that kept it for its
-backward pass raises there.  Arguments that do not fit raise ValueError before anything runs; an error of the library raises RlgpuError.
+kept between calls, so a call may be captured into a graph.  The gradients are explicit calls, not autograd nodes: outputs carry no graph, also where the
+logits require a gradient (a loss that is added to another sends its dlogits through logits.backward by itself).  What is written in place (out=, clipped
+gradients) counts as modified for autograd, as after torch's own in-place operations: a graph that kept it for its backward pass raises there.  Arguments
+that do not fit raise ValueError before anything runs; an error of the library raises RlgpuError.
 """
 import ctypes as C
 from array import array

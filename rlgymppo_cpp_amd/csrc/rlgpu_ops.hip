@@ -27,7 +27,7 @@ constexpr int64_t CACHE_BYTES = 256ll << 20, STREAM_BYTES = 2 * CACHE_BYTES;   /
 struct RowArgs {
     RlgpuPolicyRows p;
     float k, inv_t, log_floor;            // log2(e) / T, 1 / T, log(min_prob)
-    float none, near;                     // Pack::LIMIT: a logit that is no larger is not allowed; the least m that is neither far nor within CLEAR of LIMIT k
+    float near;                           // the least m that is neither far nor within CLEAR of Pack::LIMIT k
     unsigned turn;
     float *logp, *entropy;                // optional
     const float *d_logp, *d_entropy;      // backward
@@ -150,7 +150,11 @@ __device__ __forceinline__ void piece_done() { __builtin_amdgcn_sched_barrier(0)
 // A quick sum can fail where logits are far from what a policy has: e t is NaN where t is -inf, and where k x passes FAR (the mask's FILL, a caller's -1e30) the
 // rounding of m would be an exponent itself.  W is then not finite, and the lane sums again with CAREFUL: against the exact maximum, with (x - x0) k for
 // k x - m where m is far, no t below LOW, and without what is not allowed.
-constexpr float SLACK = 8.f, FAR = 1e8f, LOWEST = -3.4028234663852886e38f;
+//
+// A row whose m passes ROW_FAR, or in which FILL shows, is summed again as a whole, with EXACT: all t are (x - x0) k then.  The two kinds of t differ by the rounding of
+// m, up to 2^2 at ROW_FAR, and must not be added up as one; a lane's own choice of them, at twice ROW_FAR, is of no account in a row that is not far.
+enum Care { QUICK, CAREFUL, EXACT };
+constexpr float SLACK = 8.f, ROW_FAR = 5e7f, FAR = 2 * ROW_FAR, LOWEST = -3.4028234663852886e38f;
 constexpr float CLEAR = 160.f;            // so far under m FILL's e is 0 (float32 ends at 2^-149)
 constexpr float LOW = -1e4f;              // 2^LOW is 0, and LOW times anything that occurs is finite: an exponent below is as good as LOW
 // k x0, rounded: left to itself the compiler joins the product with the difference that it is used in, and m would have another value in every place
@@ -159,34 +163,43 @@ __device__ __forceinline__ float times_k(float x0, float k) {
     return x0 * k;
 }
 __device__ __forceinline__ bool is_far(float m) { return !(fabsf(m) < FAR); }
-__device__ __forceinline__ float exponent(float x, float k, float x0, float m) { return is_far(m) ? (x - x0) * k : fmaf(x, k, -m); }
+template <Care C> __device__ __forceinline__ float exponent(float x, float k, float x0, float m) { return C == EXACT || (C == CAREFUL && is_far(m)) ? (x - x0) * k : fmaf(x, k, -m); }
 __device__ __forceinline__ float allowed(float x, float limit) { return x <= limit ? -INFINITY : x; }                 // (a NaN stays)
-__device__ __forceinline__ bool needs_care(const RowArgs& g, float m) { return !(m >= g.near && m < FAR); }   // far, or FILL shows
-__device__ __forceinline__ float step_to(float x0, float m, float new_x0, float new_m, float k) { return fmaxf(is_far(m) || is_far(new_m) ? (x0 - new_x0) * k : m - new_m, LOW); }
+__device__ __forceinline__ bool needs_exact(const RowArgs& g, float m) { return !(m >= g.near && m < ROW_FAR); }   // far, or FILL shows
+template <Care C> __device__ __forceinline__ float step_to(float x0, float m, float new_x0, float new_m, float k) {
+    return fmaxf(C == EXACT || (C == CAREFUL && (is_far(m) || is_far(new_m))) ? (x0 - new_x0) * k : m - new_m, LOW);
+}
+// what a row's exponents are taken against: t = (x - a) k - b with a = x0 and b = 0, or a = 0 and b = m
+struct Base {
+    float a, b;
+    __device__ __forceinline__ Base(bool exact, float x0, float m) : a(exact ? x0 : 0.f), b(exact ? 0.f : m) {}
+    __device__ __forceinline__ float t(float x, float k) const { return fmaf(x - a, k, -b); }
+};
+template <Care C> using care = std::integral_constant<Care, C>;
 struct RowSum {
     float x0, m, s[2], w[2];
     __device__ __forceinline__ void clear() { x0 = LOWEST; m = -INFINITY; s[0] = s[1] = w[0] = w[1] = 0.f; }
     // `top`: the largest x of what comes next
-    template <bool CAREFUL> __device__ __forceinline__ void reach(float top, float k) {
+    template <Care C> __device__ __forceinline__ void reach(float top, float k) {
         const float to = times_k(top, k);
-        if (CAREFUL ? top > x0 : to > m + SLACK) {
-            const float by = CAREFUL ? step_to(x0, m, top, to, k) : fmaxf(m - to, LOW), f = __builtin_amdgcn_exp2f(by);
+        if (C != QUICK ? top > x0 : to > m + SLACK) {
+            const float by = step_to<C>(x0, m, top, to, k), f = __builtin_amdgcn_exp2f(by);
             for (int j = 0; j < 2; j++) { w[j] = f * fmaf(s[j], by, w[j]); s[j] *= f; }
             x0 = top; m = to;
         }
     }
-    template <bool CAREFUL, typename P> __device__ __forceinline__ void add(float x, float k, int j) {
-        if (CAREFUL) x = allowed(x, P::LIMIT);
-        const float t = CAREFUL ? exponent(x, k, x0, m) : fmaf(x, k, -m), e = __builtin_amdgcn_exp2f(t);
-        s[j] += e; w[j] = fmaf(e, CAREFUL ? fmaxf(t, LOW) : t, w[j]);
+    template <Care C, typename P> __device__ __forceinline__ void add(float x, float k, int j) {
+        if (C != QUICK) x = allowed(x, P::LIMIT);
+        const float t = exponent<C>(x, k, x0, m), e = __builtin_amdgcn_exp2f(t);
+        s[j] += e; w[j] = fmaf(e, C != QUICK ? fmaxf(t, LOW) : t, w[j]);
     }
-    template <bool CAREFUL, typename P> __device__ __forceinline__ void piece(u32x4& v, float k) {
+    template <Care C, typename P> __device__ __forceinline__ void piece(u32x4& v, float k) {
         float top = max3(P::get(v, 0), P::get(v, 1), P::get(v, 2));
 #pragma unroll
         for (int j = 3; j + 1 < P::N; j += 2) top = max3(top, P::get(v, j), P::get(v, j + 1));
-        reach<CAREFUL>(max3(top, P::get(v, P::N - 1), P::get(v, P::N - 1)), k);
+        reach<C>(max3(top, P::get(v, P::N - 1), P::get(v, P::N - 1)), k);
 #pragma unroll
-        for (int j = 0; j < P::N; j++) add<CAREFUL, P>(P::get(v, j), k, j & 1);
+        for (int j = 0; j < P::N; j++) add<C, P>(P::get(v, j), k, j & 1);
         asm("" : "+v"(v), "+v"(s[0]), "+v"(s[1]), "+v"(w[0]), "+v"(w[1]));
         piece_done();
     }
@@ -220,14 +233,14 @@ template <int G, typename OP> __device__ __forceinline__ float get_waves(const f
 
 // What follows from a row's x0, S and W and its action's logit: whether it counts, its outputs, and what its gradient needs.
 struct RowNumbers { float logp, H, lpa, L, c, h; bool on; };
-template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const RowArgs& g, const RowInputs& in, float x0, float S, float W, float xa, float (&st)[STATS]) {
+template <Mode MODE, typename P> __device__ __forceinline__ RowNumbers row_numbers(const RowArgs& g, const RowInputs& in, float x0, Base base, float S, float W, float xa, float (&st)[STATS]) {
     RowNumbers n{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, true};
-    if (!(x0 > g.none)) n.on = S != S;                    // nothing is allowed, but a NaN shows
+    if (!(x0 > P::LIMIT)) n.on = S != S;                    // nothing is allowed, but a NaN shows
     if (!n.on) return n;
     n.L = __builtin_amdgcn_logf(S);                       // (log2; S is about 1 at least)
-    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (exponent(xa, g.k, x0, times_k(x0, g.k)) - n.L);
+    const float H = LN2 * (n.L - W * __builtin_amdgcn_rcpf(S)), lpa = LN2 * (base.t(xa, g.k) - n.L);
     n.H = H < 0.f ? 0.f : H;                              // (the rounding of m can leave either an ulp of t off; a NaN stays)
-    n.lpa = xa <= g.none ? LOW : lpa > 0.f ? 0.f : (lpa < LOW ? LOW : lpa);    // (below every floor)
+    n.lpa = xa <= P::LIMIT ? LOW : lpa > 0.f ? 0.f : (lpa < LOW ? LOW : lpa);    // (below every floor)
     const bool floored = n.lpa < g.log_floor;
     n.logp = floored ? g.log_floor : n.lpa;
     if (MODE == BACKWARD) { n.c = floored ? 0.f : in.u; n.h = in.v; }
@@ -237,23 +250,23 @@ template <Mode MODE> __device__ __forceinline__ RowNumbers row_numbers(const Row
 // The gradient of a piece: e_i / S [ -c - h (H + ln2 (t_i - L)) ] / T as e_i (p0 + p1 t_i).  The action's own c / T comes in a store of its own, of the lane that
 // wrote the 16 bytes around it.
 struct RowGradient {
-    float k, x0, m, p0, p1, limit; bool careful;
-    __device__ __forceinline__ RowGradient(const RowArgs& g, const RowNumbers& n, float x0, bool careful) : k(g.k), x0(x0), m(times_k(x0, g.k)), limit(g.none) {
+    float k, p0, p1; Base base; bool careful;
+    __device__ __forceinline__ RowGradient(const RowArgs& g, const RowNumbers& n, Base base, bool careful) : k(g.k), base(base) {
         const float inv = g.inv_t * __builtin_amdgcn_exp2f(-n.L);
         p1 = -n.h * LN2 * inv; p0 = -(n.c + n.h * (n.H - LN2 * n.L)) * inv;
         // an e_i of 0 times p0 + p1 t_i is 0 while that is finite: any t_i may be -3e38
         this->careful = careful || !(fmaf(fabsf(p0), 0x1p-126f, fabsf(p1)) < 0.5f);
     }
-    __device__ __forceinline__ float quick(float x) const { const float t = fmaf(x, k, -m); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
-    __device__ __forceinline__ float of(float x) const {
-        const float t = fmaxf(exponent(x, k, x0, m), LOW);
-        return x <= limit ? 0.f : __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0);
+    __device__ __forceinline__ float quick(float x) const { const float t = fmaf(x, k, -base.b); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
+    template <typename P> __device__ __forceinline__ float of(float x) const {
+        const float t = fmaxf(base.t(x, k), LOW);
+        return x <= P::LIMIT ? 0.f : __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0);
     }
     template <typename P> __device__ __forceinline__ u32x4 piece(u32x4 q) const {
         float d[P::N];
         if (careful) {
 #pragma unroll
-            for (int j = 0; j < P::N; j++) d[j] = of(P::get(q, j));
+            for (int j = 0; j < P::N; j++) d[j] = of<P>(P::get(q, j));
         } else {
 #pragma unroll
             for (int j = 0; j < P::N; j++) d[j] = quick(P::get(q, j));
@@ -310,7 +323,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
         const bool here = row < g.p.rows;
         auto one = [&](int i) -> float { return masked && !mask[i] ? P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0) : (float)x[i]; };
         auto piece = [&](int c) -> u32x4 { u32x4 q = load<STREAM>(x + c * N); if (masked) q = P::forbid(q, P::bytes(mask + c * N)); return q; };
-        float x0 = 0.f;
+        Base base(false, 0.f, 0.f);
         RowNumbers n{};
         float xt = P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
         bool careful = false;
@@ -331,25 +344,25 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
                 for (int i = 0; i < NV; i++) { v[i] = P::forbid(v[i], b[i]); piece_done(); }
             }
             RowSum r;
-            auto sum = [&](auto careful) {
-                constexpr bool CAREFUL = decltype(careful)::value;
+            auto sum = [&](auto care) {
+                constexpr Care C = decltype(care)::value;
 #pragma unroll
-                for (int i = 0; i < NV; i++) r.template piece<CAREFUL, P>(v[i], k);
+                for (int i = 0; i < NV; i++) r.template piece<C, P>(v[i], k);
                 if (MORE)
                     for (int p = lane + NV * G; p < whole; p += BATCH * G) {
                         u32x4 q[BATCH];
 #pragma unroll
                         for (int i = 0; i < BATCH; i++) { q[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; if (p + i * G < whole) q[i] = piece(p + i * G); }
 #pragma unroll
-                        for (int i = 0; i < BATCH; i++) r.template piece<CAREFUL, P>(q[i], k);
+                        for (int i = 0; i < BATCH; i++) r.template piece<C, P>(q[i], k);
                     }
-                r.template reach<CAREFUL>(xt, k);
-                r.template add<CAREFUL, P>(xt, k, 1);
+                r.template reach<C>(xt, k);
+                r.template add<C, P>(xt, k, 1);
             };
             r.clear();
-            sum(std::false_type{});
+            sum(care<QUICK>{});
             careful = !(fabsf(r.W()) < INFINITY);
-            if (careful) { r.clear(); sum(std::true_type{}); }
+            if (careful) { r.clear(); sum(care<CAREFUL>{}); }
             // the lanes' sums against the row's x0
             auto largest = [&]() {
                 if (G <= 64) return lanes<G, Max>(r.x0);
@@ -357,17 +370,19 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
                 __syncthreads();
                 return get_waves<G, Max>(red[0]);
             };
-            x0 = largest();
-            float m = times_k(x0, k), by;
-            if (needs_care(g, m)) {
+            float x0 = largest(), by;
+            const float m = times_k(x0, k);
+            const bool exact = needs_exact(g, m);
+            if (exact) {
                 careful = true;
                 // (two of a far row's largest may be one exponent once rounded: the x0 of the quick sums need not be the larger)
                 r.clear();
-                sum(std::true_type{});
+                sum(care<EXACT>{});
                 if (G > 64) __syncthreads();
-                x0 = largest(); m = times_k(x0, k);
-                by = step_to(r.x0, r.m, x0, m, k);
-            } else by = fmaxf(r.m - m, LOW);
+                x0 = largest();
+                by = step_to<EXACT>(r.x0, r.m, x0, m, k);
+            } else by = step_to<QUICK>(r.x0, r.m, x0, m, k);
+            base = Base(exact, x0, m);
             const float f = __builtin_amdgcn_exp2f(by);
             // (scaled first: a lane that has nothing but a caller's -1e9 can hold an S of up to 2^127, whose product with `by` is not finite)
             float S = f * r.S(), Wt = fmaf(S, by, f * r.W());
@@ -378,7 +393,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
                 S = get_waves<G, Sum>(red[1]); Wt = get_waves<G, Sum>(red[2]);
             }
             float st[STATS];
-            n = row_numbers<MODE>(g, in, x0, S, Wt, xa, st);
+            n = row_numbers<MODE, P>(g, in, x0, base, S, Wt, xa, st);
             on = n.on;
             // (a lane for each statistic; added in LDS, so that no sum is in a register: nobody else adds to it)
             if (MODE == LOSS && on && lane < STATS) {
@@ -403,7 +418,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
                 if (lane < rest) dx[whole * N + lane] = (T)0.f;
             }
         } else {
-            const RowGradient d(g, n, x0, careful);
+            const RowGradient d(g, n, base, careful);
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 if (lane < whole - i * G) store<STREAM>((char*)dx + i * G * 16 + at, d.template piece<P>(v[i]));
@@ -418,7 +433,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
 #pragma unroll
                     for (int i = 0; i < BATCH; i++) { if (p + i * G < whole) store<STREAM>(dx + (p + i * G) * N, d.template piece<P>(q[i])); piece_done(); }
                 }
-            if (lane < rest) dx[whole * N + lane] = (T)d.of(xt);
+            if (lane < rest) dx[whole * N + lane] = (T)d.template of<P>(xt);
             const int pa = a / N;
             if (lane == (pa < whole ? pa % G : a - whole * N)) dx[a] = (T)RowGradient::action(g, n);
         }
@@ -434,7 +449,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, G == 512 ? 4 : MODE == BACK
 }
 
 // ---- few rows of many actions: a row over `splits` workgroups, `per` pieces each ---------------------------------------------------------------------------
-// k_parts leaves x0, S and W of its part in part[row][split] and the action's logit behind the row's parts (the gradient may overwrite it before another part of
+// k_parts leaves x0, S (negative where the sums are EXACT) and W of its part in part[row][split] and the action's logit behind the row's parts (the gradient may overwrite it before another part of
 // the row is done); k_join adds a row's parts up in every workgroup that needs them and writes the outputs and its part of the gradient.  (Those workgroups join in
 // the same order; the one of the loss's statistics has fewer lanes for a row and another order, and its last bits may not be those of logp and the gradient.)
 struct SplitArgs { int splits, per; float* part; };      // part: [rows][3 * splits + 1]
@@ -462,47 +477,54 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_parts(
     if (split == 0 && lane == 0) part[3 * sp.splits] = r.one(a);
     const float xt = lane < r.rest ? r.one(r.whole * P::N + lane) : P::get(u32x4{P::FILL, P::FILL, P::FILL, P::FILL}, 0);
     RowSum s;
-    auto sum = [&](auto careful) {
-        constexpr bool CAREFUL = decltype(careful)::value;
+    auto sum = [&](auto care) {
+        constexpr Care C = decltype(care)::value;
         for (int p = r.from + lane; p < r.to; p += 4 * 256) {
             u32x4 q[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) { q[i] = u32x4{P::FILL, P::FILL, P::FILL, P::FILL}; if (p + i * 256 < r.to) q[i] = r.piece(p + i * 256); }
 #pragma unroll
-            for (int i = 0; i < 4; i++) s.template piece<CAREFUL, P>(q[i], g.k);
+            for (int i = 0; i < 4; i++) s.template piece<C, P>(q[i], g.k);
         }
-        s.template reach<CAREFUL>(xt, g.k);
-        s.template add<CAREFUL, P>(xt, g.k, 1);
+        s.template reach<C>(xt, g.k);
+        s.template add<C, P>(xt, g.k, 1);
     };
     s.clear();
-    sum(std::false_type{});
-    if (!(fabsf(s.W()) < INFINITY)) { s.clear(); sum(std::true_type{}); }
+    sum(care<QUICK>{});
+    if (!(fabsf(s.W()) < INFINITY)) { s.clear(); sum(care<CAREFUL>{}); }
     auto largest = [&]() { put_wave<256, Max>(s.x0, red[0]); __syncthreads(); return get_waves<256, Max>(red[0]); };
-    float x0 = largest(), m = times_k(x0, g.k), by;
-    if (needs_care(g, m)) {                 // (as in k_rows)
+    float x0 = largest(), by;
+    const float m = times_k(x0, g.k);
+    const bool exact = needs_exact(g, m);
+    if (exact) {                                          // (as in k_rows)
         s.clear();
-        sum(std::true_type{});
+        sum(care<EXACT>{});
         __syncthreads();
-        x0 = largest(); m = times_k(x0, g.k);
-        by = step_to(s.x0, s.m, x0, m, g.k);
-    } else by = fmaxf(s.m - m, LOW);
+        x0 = largest();
+        by = step_to<EXACT>(s.x0, s.m, x0, m, g.k);
+    } else by = step_to<QUICK>(s.x0, s.m, x0, m, g.k);
     const float f = __builtin_amdgcn_exp2f(by);
     put_wave<256, Sum>(f * s.S(), red[1]); put_wave<256, Sum>(fmaf(f * s.S(), by, f * s.W()), red[2]);
     __syncthreads();
     const float S = get_waves<256, Sum>(red[1]), W = get_waves<256, Sum>(red[2]);
-    if (lane == 0) { part[split] = x0; part[sp.splits + split] = S; part[2 * sp.splits + split] = W; }
+    if (lane == 0) { part[split] = x0; part[sp.splits + split] = exact ? -S : S; part[2 * sp.splits + split] = W; }
 }
 // the parts of a row joined by `n` lanes, of which this is `at`
-__device__ __forceinline__ void join(const RowArgs& g, const SplitArgs& sp, const float* part, int at, int n, float& x0, float& S, float& W) {
+__device__ __forceinline__ Base join(const RowArgs& g, const SplitArgs& sp, const float* part, int at, int n, float& x0, float& S, float& W) {
     x0 = LOWEST; S = W = 0.f;
     for (int i = at; i < sp.splits; i += n) x0 = fmaxf(x0, part[i]);
     for (int o = n >> 1; o > 0; o >>= 1) x0 = fmaxf(x0, __shfl_xor(x0, o, 64));
     const float m = times_k(x0, g.k);
+    const Base base(needs_exact(g, m), x0, m);
     for (int i = at; i < sp.splits; i += n) {
-        const float by = step_to(part[i], times_k(part[i], g.k), x0, m, g.k), f = __builtin_amdgcn_exp2f(by), Si = part[sp.splits + i];
-        S += f * Si; W += f * fmaf(Si, by, part[2 * sp.splits + i]);
+        const float at_x0 = part[i], Si = part[sp.splits + i];
+        const Base of(signbit(Si), at_x0, times_k(at_x0, g.k));
+        // the step between two bases, of either kind, without the rounding of any m
+        const float by = fmaxf(fmaf(of.a - base.a, g.k, of.b - base.b), LOW), f = __builtin_amdgcn_exp2f(by), size = fabsf(Si);
+        S += f * size; W += f * fmaf(size, by, part[2 * sp.splits + i]);
     }
     for (int o = n >> 1; o > 0; o >>= 1) { S += __shfl_xor(S, o, 64); W += __shfl_xor(W, o, 64); }
+    return base;
 }
 // The loss's statistics, by one workgroup beside those that write the gradient: 2 to 64 lanes a row, so that all rows are joined at once, then a sum over them in
 // 64 bits.  (A launch behind this one takes 3 us more, and 4 us more of the call.)
@@ -517,8 +539,8 @@ template <typename T> __device__ __forceinline__ void split_stats(const RowArgs&
         if (row_counts<T, LOSS>(g, row, a, w)) {
             const float* const part = sp.part + (int64_t)row * (3 * sp.splits + 1);
             float x0, S, W;
-            join(g, sp, part, at, n, x0, S, W);
-            on = row_numbers<LOSS>(g, row_inputs<LOSS>(g, row, w), x0, S, W, part[3 * sp.splits], mine).on;
+            const Base base = join(g, sp, part, at, n, x0, S, W);
+            on = row_numbers<LOSS, Pack<T>>(g, row_inputs<LOSS>(g, row, w), x0, base, S, W, part[3 * sp.splits], mine).on;
         }
         if (at == 0) for (int j = 0; j < STATS; j++) st[row][j] = on ? mine[j] : 0.f;
     }
@@ -537,7 +559,8 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(R
         return;
     }
     const SplitRow<T> r(g, sp, row, split);
-    int a; float w, x0 = LOWEST;
+    int a; float w;
+    Base base(false, 0.f, 0.f);
     RowNumbers n{};
     // (the first pieces are asked for before the parts are joined)
     constexpr int BATCH = 4;
@@ -550,9 +573,9 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(R
     if (grad) fetch(r.from + lane);
     if (row_counts<T, MODE>(g, row, a, w)) {
         const float* const part = sp.part + (int64_t)row * (3 * sp.splits + 1);
-        float S, W, st[STATS];
-        join(g, sp, part, lane & 63, 64, x0, S, W);
-        n = row_numbers<MODE>(g, row_inputs<MODE>(g, row, w), x0, S, W, part[3 * sp.splits], st);
+        float x0, S, W, st[STATS];
+        base = join(g, sp, part, lane & 63, 64, x0, S, W);
+        n = row_numbers<MODE, P>(g, row_inputs<MODE>(g, row, w), x0, base, S, W, part[3 * sp.splits], st);
     }
     if (split == 0 && lane == 0) {
         if (g.logp) g.logp[row] = n.logp;
@@ -560,13 +583,13 @@ template <typename T, Mode MODE> __global__ void __launch_bounds__(256) k_join(R
     }
     if (!grad) return;
     T* const dx = (T*)g.dlogits + row_offset(row, g.ldd);
-    const RowGradient d(g, n, x0, true);
+    const RowGradient d(g, n, base, true);
     for (int p = r.from + lane; p < r.to; p += BATCH * 256) {
         if (p != r.from + lane) fetch(p);
 #pragma unroll
         for (int i = 0; i < BATCH; i++) if (p + i * 256 < r.to) store<false>(dx + (p + i * 256) * P::N, n.on ? d.template piece<P>(q[i]) : u32x4{0, 0, 0, 0});
     }
-    if (lane < r.rest) dx[r.whole * P::N + lane] = (T)(n.on ? d.of(r.one(r.whole * P::N + lane)) : 0.f);
+    if (lane < r.rest) dx[r.whole * P::N + lane] = (T)(n.on ? d.template of<P>(r.one(r.whole * P::N + lane)) : 0.f);
     if (!n.on) return;
     const int pa = a / P::N;
     if (pa < r.whole ? pa >= r.from && pa < r.to && lane == (pa - r.from) % 256 : lane == a - r.whole * P::N && lane < r.rest) dx[a] = (T)RowGradient::action(g, n);
@@ -807,7 +830,7 @@ template <typename T, Mode MODE> int launch_split(RowArgs& g, hipStream_t s, int
 template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM = false> int launch_rows_as(RowArgs& g, hipStream_t s, int& blocks) {
     constexpr int threads = G <= 64 ? 256 : G, rpb = threads / G;
     // (512 lanes of a loss: two workgroups a CU and not three, 201 and 212 us for 12 201 rows of 11 000 float32 actions)
-    constexpr int waves = MODE == LOGP || (MODE == BACKWARD && G <= 16) ? 8 : MODE == BACKWARD && G <= 64 ? 7 : MODE == LOSS && G == 512 ? 4 : 6;
+    constexpr int waves = MODE == LOGP || (MODE == BACKWARD && G <= 16) ? 8 : MODE == BACKWARD && G <= 64 && NV < 6 ? 7 : MODE == LOSS && G == 512 ? 4 : 6;
     static const int most = resident(&k_rows<T, G, NV, MODE, MORE, STREAM>, threads, waves);
     const int groups = (g.p.rows + rpb - 1) / rpb, passes = (groups + most - 1) / most;
     blocks = (groups + passes - 1) / passes;              // as many rows for each (2 048 groups: 1 024 workgroups twice, 12.1 us, not 1 536 and then 512, 12.5)
@@ -822,7 +845,7 @@ template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM = false> 
 // Lanes and 16-byte pieces a row: the smallest set of registers that holds it.  Sums alone need no more of a row than what is in flight: 256 lanes take any.
 template <typename T, Mode MODE> int launch_rows_of(RowArgs g, hipStream_t s, int& blocks) {
     const int whole = g.p.n_actions / Pack<T>::N;
-    g.none = Pack<T>::LIMIT; g.near = std::max(g.none * g.k + CLEAR, -FAR);
+    g.near = std::max(Pack<T>::LIMIT * g.k + CLEAR, -ROW_FAR);
     const int splits = splits_for(g.p.dtype, g.p.rows, g.p.n_actions);
     if (splits > 1) return launch_split<T, MODE>(g, s, splits, blocks);
     if (whole <= 8) return launch_rows_as<T, 8, 1, MODE, false>(g, s, blocks);

@@ -109,6 +109,20 @@ def test_largest_values_of_one_rounded_exponent(A, rows, base, temperature):
     check_row_calls(x, act.to(torch.int32), None, temperature, g, some=torch.randperm(rows, generator=g)[:64].sort().values if A > 5000 else None)
 
 
+@gpu
+@pytest.mark.parametrize("temperature", [1.0, 1.25, 0.6, 1e-3])
+@pytest.mark.parametrize("border", [1e8, -1e8, 5e7, -5e7])
+@pytest.mark.parametrize("A,rows", [(60, 300), (700, 60), (9000, 9), (40000, 9), (40000, 130)])
+def test_rows_across_the_border_of_far(A, rows, border, temperature):
+    """Exponents within a few steps of where they count as far, on both sides of it in one row, in one lane, in one part."""
+    g = torch.Generator().manual_seed(A)
+    x = torch.full((rows, A), border / math.log2(math.e) * temperature, dtype=torch.float64)
+    ulp = abs(float(torch.nextafter(x[0, 0].float(), torch.tensor(math.inf))) - float(x[0, 0].float()))
+    x = (x + ulp * torch.randint(-3, 4, (rows, 1), generator=g) - ulp * torch.randint(0, 3, (rows, A), generator=g)).float()
+    act = torch.randint(0, A, (rows,), generator=g).to(torch.int32)
+    check_row_calls(x, act, None, temperature, g, some=torch.randperm(rows, generator=g)[:64].sort().values if A > 5000 else None)
+
+
 # ---- temperatures at which a type's lowest value is an ordinary exponent ------------------------------------------------------------------------------------
 
 @gpu

@@ -90,7 +90,7 @@ using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 
 // N values of T in 16 bytes.  An action that is not allowed and places behind a row's end hold FILL (as a number LIMIT: -9.97e36; float16: its lowest value, -65504):
 // finite (an e t of 0 times -inf would be NaN), and 0 in any sum as long as its exponent is CLEAR of the row's.  Where it is not (a row's logits are next to it, or
-// the temperature makes it an ordinary exponent: float16 from T of about 590 on) CAREFUL sums leave it out by its value.  A caller's own logits of LIMIT or less
+// the temperature makes it an ordinary exponent: float16 from T of about 590 on) CAREFUL and EXACT sums leave it out by its value.  A caller's own logits of LIMIT or less
 // are so left out too: they are masks.
 template <typename T> struct Pack;
 template <> struct Pack<float> {
@@ -141,7 +141,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm(
 
 // Between two pieces of a row.  Left alone, the scheduler unpacks every piece first and adds later, as the sums are one long chain, or keeps the 32-bit values of
 // one pass for the next (219 registers where 32 hold a row in 16 bits).  The sets of 16 pieces a lane are at the limit of 128 registers all the same: their gradient
-// spills 4 to 6 in 16 bits, the loss 8 to 10 in float32 and 20 to 23 in 16 bits, once a row.
+// spills 4 to 6 in 16 bits, the loss 4 to 10 in float32 and 20 to 23 in 16 bits, once a row.
 __device__ __forceinline__ void piece_done() { __builtin_amdgcn_sched_barrier(0); }
 
 // What a lane has of S and W.  `m` is the exponent (k x0) that its sums are taken against: not the maximum, but within SLACK of it, so that it hardly ever moves
@@ -283,7 +283,7 @@ struct RowGradient {
 // the same places do not leave some workgroups all the padding.  With 1024 lanes only one workgroup fits a CU, and it asks for its next row's pieces as it
 // writes the last's gradient: otherwise memory would wait for the sums and the sums for memory.
 //
-// Wavefronts a SIMD are asked for where they pay: 8 for the gradient of short rows (in 16 bits 2 to 8 registers spill for it: 1.5 M rows of 90 float16 actions 166 us
+// Wavefronts a SIMD are asked for where they pay: 8 for the gradient of short rows (in 16 bits 2 to 6 registers spill for it: 1.5 M rows of 90 float16 actions 166 us
 // against 190 without, 1 M of 128 116 and 128, but 335 544 of 400 124 and 119), 6 for the loss of up to 3 pieces a lane (one register fewer: 191 739 rows of 700
 // bfloat16 actions 124 and 128 us).
 template <typename T, int G, int NV, Mode MODE, bool MORE, bool STREAM>

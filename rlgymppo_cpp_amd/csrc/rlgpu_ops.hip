@@ -259,8 +259,9 @@ struct RowGradient {
     }
     __device__ __forceinline__ float quick(float x) const { const float t = fmaf(x, k, -base.b); return __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0); }
     template <typename P> __device__ __forceinline__ float of(float x) const {
-        const float t = fmaxf(base.t(x, k), LOW);
-        return x <= P::LIMIT ? 0.f : __builtin_amdgcn_exp2f(t) * fmaf(p1, t, p0);
+        // (e first: an e of 0 leaves nothing of a p1 t that is not finite)
+        const float t = fmaxf(base.t(x, k), LOW), e = __builtin_amdgcn_exp2f(t);
+        return x <= P::LIMIT ? 0.f : fmaf(e * p1, t, e * p0);
     }
     template <typename P> __device__ __forceinline__ u32x4 piece(u32x4 q) const {
         float d[P::N];

@@ -183,6 +183,22 @@ def test_temperatures_near_the_largest_number(A, rows, dt, masked):
 
 
 @gpu
+@pytest.mark.parametrize("how", ["mask", "-inf", "-1e20", "none"])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("A,rows", [(6, 9), (90, 9), (1003, 9), (20011, 9), (50021, 9)])
+def test_temperatures_near_the_smallest_number(A, rows, dt, how):
+    """Gradients of 1 / T = 10^35 beside actions that have no probability at all: those get 0."""
+    for temperature in (1e-30, 1e-35, 2.3e-36):
+        _, x, act, mask, g = make(rows, A, DTYPES[dt], seed=15, masked=True)
+        x = (x.float() * temperature).to(DTYPES[dt])
+        x[:, 0] -= 1e-20                                    # (far below, whatever the mask)
+        if how in ("-inf", "-1e20"):
+            x = torch.where(mask, x, torch.full_like(x, float(how)))
+        act[act == 0] = A - 1
+        check_row_calls(x, act, mask if how == "mask" else None, temperature, g, size=0.5)
+
+
+@gpu
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("A", [90, 700, 40000])
 def test_where_a_row_begins_to_count(A, dt):
